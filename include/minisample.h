@@ -306,6 +306,102 @@ int ms_merge_records(ms_ctx* ctx, const void* records, int64_t B, int64_t G, int
                      const ms_params* params, const double* u, int32_t* out_ids, ms_diag* diag,
                      int64_t rec_bytes, void* stream);
 
+/*
+ * Scoring a [B, V] block of logits: what a server returns beside the ids that
+ * ms_sample drew, and what training on those ids or on another model's top ids
+ * needs.  No reference counterpart: the reference returns ids only
+ * (src/generation.js:71-81).
+ *
+ * All three calls take device pointers on the context's first device, run on
+ * `stream` (NULL = the ctx stream) asynchronously, keep nothing between calls
+ * and use no scratch memory: calls on several streams, and captured and
+ * replayed ones, do not disturb one another.
+ *
+ * Common arguments:
+ *   logits   [B, ld] of `dtype` (MS_F32, MS_BF16 or MS_F16), ld >= V (row
+ *            stride in elements; ignored for B = 1), aligned to an element;
+ *            1 <= V <= 65535 * 16384, B <= 2^31 - 1
+ *   temperature  z = logits / temperature; 0.0001 < temperature <= 10000
+ *   a -Inf logit is an id that cannot be chosen: probability 0
+ * Rows without a distribution:
+ *   a NaN or +Inf logit: the row's outputs and gradients are NaN, its ids -1
+ *   every logit -Inf: log-probabilities -Inf, entropy 0, no alternatives,
+ *     distillation loss +Inf, gradients 0
+ */
+#define MS_F32  0
+#define MS_BF16 1
+#define MS_F16  2
+
+/* Outputs of ms_logprobs; each pointer may be NULL. */
+typedef struct ms_scores {
+    float*   logprobs;      /* [B, n_tokens] */
+    float*   entropy;       /* [B] -sum p log p (nats) */
+    int32_t* top_ids;       /* [B, top_n] */
+    float*   top_logprobs;  /* [B, top_n] */
+    double*  row_max;       /* [B] max of z, as in ms_diag */
+    double*  row_sum;       /* [B] sum of exp(z - row_max): log-sum-exp = row_max + log(row_sum) */
+} ms_scores;
+
+/*
+ * Log-probabilities of given ids, the entropy and the top alternatives of every
+ * row, under softmax(z).
+ *   tokens   [B, n_tokens] int32, 0 <= n_tokens <= 256 (NULL when 0).  An id
+ *            outside [0, V) is no token: its log-probability is 0.  A row all
+ *            of whose tokens are such is padding (n_tokens > 0): its logits are
+ *            not read, its outputs are 0, its alternatives -1 / -Inf.
+ *   top_n    0 <= top_n <= 256: the ids of the largest logits, largest first,
+ *            equal logits by ascending id; -Inf logits are never listed, places
+ *            without an alternative hold -1 / -Inf
+ */
+int ms_logprobs(ms_ctx* ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t ld, double temperature,
+                const int32_t* tokens, int32_t n_tokens, int32_t top_n, const ms_scores* out, void* stream);
+
+/*
+ * Gradient of the logits from those of the log-probabilities and the entropy:
+ *   dlogits_i = (1/temperature) [ sum_t g_t [i = token_t] - p_i (G + g_H (log p_i + H)) ],  G = sum_t g_t
+ *   row_max, row_sum   [B], as ms_logprobs wrote them for the same logits,
+ *            tokens and temperature
+ *   g_logprobs  [B, n_tokens] or NULL (0); read only where the token is one
+ *   g_entropy   [B] or NULL (0); needs entropy [B] (NULL without it)
+ *   dlogits  [B, dld] of `dtype`, dld >= V; may be `logits` itself (dld = ld),
+ *            and must not overlap it otherwise
+ * Padding rows, rows of -Inf alone and rows whose gradients are all 0 get 0.
+ */
+int ms_logprobs_backward(ms_ctx* ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t ld,
+                         double temperature, const int32_t* tokens, int32_t n_tokens, const double* row_max,
+                         const double* row_sum, const float* entropy, const float* g_logprobs,
+                         const float* g_entropy, void* dlogits, int64_t dld, void* stream);
+
+/*
+ * Distillation: the divergence of the student's softmax(z) from a teacher known
+ * by its top ids, and its gradient, from one read of the logits.
+ *   ids, values  [B, K] int32 / float, 1 <= K <= 256; an id outside [0, V) is
+ *            absent, and a row without a present id is padding (loss 0,
+ *            gradient 0, logits not read)
+ *   kind     MS_TEACHER_LOGITS: values are the teacher's logits; its
+ *              probabilities are q = softmax(values / temperature) over the
+ *              present ids (a value of -Inf is absent), and rest = 0
+ *            MS_TEACHER_LOGPROBS: values are the teacher's log-probabilities at
+ *              this temperature (ms_logprobs' top_logprobs), q = exp(values);
+ *              what is left, rest = 1 - sum q (0 below 2^-20, which fp32
+ *              log-probabilities do not resolve), is held against all the mass
+ *              R that the student gives to the ids not listed
+ *   loss     [B] or NULL: sum_j q_j (log q_j - log p_(ids_j)) + rest (log rest - log R)
+ *   weight   [B] or NULL (1): dlogits is weight times the gradient of loss; a
+ *            row of weight 0 gets gradient 0.  loss is not weighted.
+ *   dlogits  [B, dld] of `dtype` or NULL; as for ms_logprobs_backward
+ * An id that is listed twice has the sum of both masses; the student's
+ * probability of it counts once.
+ */
+#define MS_TEACHER_LOGITS   0
+#define MS_TEACHER_LOGPROBS 1
+int ms_distill(ms_ctx* ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t ld, double temperature,
+               const int32_t* ids, const float* values, int32_t K, int kind, const float* weight, float* loss,
+               void* dlogits, int64_t dld, void* stream);
+
+/* The CUDA device that a context's device-pointer calls run on (its first). */
+int ms_device(ms_ctx* ctx, int* device);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,5 +8,5 @@ NVCC="${NVCC:-nvcc}"
 "$NVCC" -O3 -std=c++17 -gencode arch=compute_100a,code=sm_100a -lineinfo \
   -Xcompiler -fPIC -Xcompiler -Wall -shared \
   ${MS_NVCC_EXTRA:-} \
-  "$HERE/ms_kernels.cu" "$HERE/ms_api.cu" -o "$OUT" -lcudart
+  "$HERE/ms_kernels.cu" "$HERE/ms_scores.cu" "$HERE/ms_api.cu" -o "$OUT" -lcudart
 echo "$OUT"

@@ -12,6 +12,8 @@
 #include <vector>
 
 #include "ms_device.cuh"
+#include "ms_scores.cuh"
+#include "ms_scores_args.h"
 
 namespace ms {
 cudaError_t launch_sample(const Args& A, cudaStream_t stream, cudaEvent_t* ev, int64_t* launched);
@@ -787,6 +789,130 @@ extern "C" int ms_merge_records(ms_ctx* ctx, const void* records, int64_t B, int
     A.d_row_flags = diag->row_flags;
   }
   MS_CUDA(ctx, ms::launch_merge(A, st));
+  s.launches += 1;
+  return MS_OK;
+}
+
+// ---------------------------------------------------------------- scoring
+namespace {
+
+// Makes the context's device current for a launch and the caller's again after it.
+struct OnDevice {
+  int prev = 0;
+  cudaError_t err;
+  explicit OnDevice(int device) {
+    cudaGetDevice(&prev);
+    err = prev == device ? cudaSuccess : cudaSetDevice(device);
+  }
+  ~OnDevice() {
+    int now = prev;
+    cudaGetDevice(&now);
+    if (now != prev) cudaSetDevice(prev);
+  }
+};
+
+}  // namespace
+
+extern "C" int ms_device(ms_ctx* c, int* device) {
+  if (!c || !device) return MS_ERR_ARG;
+  *device = c->devs[0].device;
+  return MS_OK;
+}
+
+extern "C" int ms_logprobs(ms_ctx* ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t ld,
+                           double temperature, const int32_t* tokens, int32_t n_tokens, int32_t top_n,
+                           const ms_scores* out, void* stream) {
+  if (!ctx) return MS_ERR_ARG;
+  if (const char* e = ms::bad_logprobs(logits, dtype, B, V, ld, temperature, tokens, n_tokens, top_n, out))
+    return fail(ctx, MS_ERR_ARG, "ms_logprobs: %s", e);
+  if (B == 0) return MS_OK;
+  DevState& s = ctx->devs[0];
+  ms::ScoreArgs A;
+  memset(&A, 0, sizeof A);
+  A.x = logits;
+  A.B = B;
+  A.V = (int32_t)V;
+  A.ld = B > 1 ? ld : V;
+  A.T = temperature;
+  A.rT = 1.0 / temperature;
+  A.a = (float)(1.4426950408889634 / temperature);
+  A.tokens = tokens;
+  A.n_tok = n_tokens;
+  A.out = *out;
+  A.top_n = (out->top_ids || out->top_logprobs) ? top_n : 0;
+  OnDevice on(s.device);
+  MS_CUDA(ctx, on.err);
+  MS_CUDA(ctx, ms::launch_logprobs(A, dtype, stream ? (cudaStream_t)stream : s.stream));
+  s.launches += 1;
+  return MS_OK;
+}
+
+extern "C" int ms_logprobs_backward(ms_ctx* ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t ld,
+                                    double temperature, const int32_t* tokens, int32_t n_tokens,
+                                    const double* row_max, const double* row_sum, const float* entropy,
+                                    const float* g_logprobs, const float* g_entropy, void* dlogits, int64_t dld,
+                                    void* stream) {
+  if (!ctx) return MS_ERR_ARG;
+  if (const char* e = ms::bad_logprobs_backward(logits, dtype, B, V, ld, temperature, tokens, n_tokens, row_max, row_sum,
+                                                  entropy, g_logprobs, g_entropy, dlogits, dld))
+    return fail(ctx, MS_ERR_ARG, "ms_logprobs_backward: %s", e);
+  if (B == 0) return MS_OK;
+  if (ms::logprobs_backward_blocks(B, (int32_t)V, dtype) > INT32_MAX)
+    return fail(ctx, MS_ERR_ARG, "ms_logprobs_backward: B * V too large for one call");
+  DevState& s = ctx->devs[0];
+  ms::ScoreArgs A;
+  memset(&A, 0, sizeof A);
+  A.x = logits;
+  A.B = B;
+  A.V = (int32_t)V;
+  A.ld = B > 1 ? ld : V;
+  A.T = temperature;
+  A.rT = 1.0 / temperature;
+  A.a = (float)(1.4426950408889634 / temperature);
+  A.tokens = tokens;
+  A.n_tok = n_tokens;
+  A.row_max = row_max;
+  A.row_sum = row_sum;
+  A.entropy = entropy;
+  A.g_lp = g_logprobs;
+  A.g_ent = g_entropy;
+  A.dx = dlogits;
+  A.dld = B > 1 ? dld : V;
+  OnDevice on(s.device);
+  MS_CUDA(ctx, on.err);
+  MS_CUDA(ctx, ms::launch_logprobs_backward(A, dtype, stream ? (cudaStream_t)stream : s.stream));
+  s.launches += 1;
+  return MS_OK;
+}
+
+extern "C" int ms_distill(ms_ctx* ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t ld,
+                          double temperature, const int32_t* ids, const float* values, int32_t K, int kind,
+                          const float* weight, float* loss, void* dlogits, int64_t dld, void* stream) {
+  if (!ctx) return MS_ERR_ARG;
+  if (const char* e = ms::bad_distill(logits, dtype, B, V, ld, temperature, ids, values, K, kind, loss, dlogits, dld))
+    return fail(ctx, MS_ERR_ARG, "ms_distill: %s", e);
+  if (B == 0) return MS_OK;
+  DevState& s = ctx->devs[0];
+  ms::DistillArgs A;
+  memset(&A, 0, sizeof A);
+  A.x = logits;
+  A.B = B;
+  A.V = (int32_t)V;
+  A.ld = B > 1 ? ld : V;
+  A.T = temperature;
+  A.rT = 1.0 / temperature;
+  A.a = (float)(1.4426950408889634 / temperature);
+  A.ids = ids;
+  A.values = values;
+  A.K = K;
+  A.kind = kind;
+  A.weight = weight;
+  A.loss = loss;
+  A.dx = dlogits;
+  A.dld = B > 1 ? dld : V;
+  OnDevice on(s.device);
+  MS_CUDA(ctx, on.err);
+  MS_CUDA(ctx, ms::launch_distill(A, dtype, stream ? (cudaStream_t)stream : s.stream));
   s.launches += 1;
   return MS_OK;
 }

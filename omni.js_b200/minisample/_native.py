@@ -35,6 +35,14 @@ MS_ROW_SLOWPATH = 0x8
 MS_ROW_UNSETTLED = 0x10
 MS_ROW_TIMEOUT = 0x20
 
+# element types, teacher kinds and the largest list of the scoring calls
+MS_F32 = 0
+MS_BF16 = 1
+MS_F16 = 2
+MS_TEACHER_LOGITS = 0
+MS_TEACHER_LOGPROBS = 1
+MS_SCORE_MAX = 256
+
 MS_INJECT_WAIT = 1
 MS_INJECT_ALLOC = 2
 ABI_VERSION = 2
@@ -48,7 +56,8 @@ ERROR_NAMES = {
 # Every symbol include/minisample.h declares.
 EXPORTED = ("ms_version", "ms_create", "ms_destroy", "ms_last_error", "ms_sample", "ms_profile_read",
             "ms_scratch_bytes", "ms_sample_noalloc", "ms_launch_count", "ms_shard_record_bytes",
-            "ms_shard_records", "ms_merge_records", "ms_debug_inject", "ms_debug_exp", "ms_history_append")
+            "ms_shard_records", "ms_merge_records", "ms_debug_inject", "ms_debug_exp", "ms_history_append",
+            "ms_logprobs", "ms_logprobs_backward", "ms_distill", "ms_device")
 
 
 class MsParams(ctypes.Structure):
@@ -73,6 +82,17 @@ class MsDiag(ctypes.Structure):
         ("row_flags", ctypes.c_void_p),
         ("pen_logits", ctypes.c_void_p),
         ("pen_ld", ctypes.c_int64),
+    ]
+
+
+class MsScores(ctypes.Structure):
+    _fields_ = [
+        ("logprobs", ctypes.c_void_p),
+        ("entropy", ctypes.c_void_p),
+        ("top_ids", ctypes.c_void_p),
+        ("top_logprobs", ctypes.c_void_p),
+        ("row_max", ctypes.c_void_p),
+        ("row_sum", ctypes.c_void_p),
     ]
 
 
@@ -143,6 +163,16 @@ def load(path: str | None = None):
         ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
         ctypes.POINTER(MsParams), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
     ]
+    vp, i32, i64, f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_double
+    block = [vp, vp, ctypes.c_int, i64, i64, i64, f64]  # ctx, logits, dtype, B, V, ld, temperature
+    L.ms_logprobs.restype = ctypes.c_int
+    L.ms_logprobs.argtypes = block + [vp, i32, i32, ctypes.POINTER(MsScores), vp]
+    L.ms_logprobs_backward.restype = ctypes.c_int
+    L.ms_logprobs_backward.argtypes = block + [vp, i32, vp, vp, vp, vp, vp, vp, i64, vp]
+    L.ms_distill.restype = ctypes.c_int
+    L.ms_distill.argtypes = block + [vp, vp, i32, ctypes.c_int, vp, vp, vp, i64, vp]
+    L.ms_device.restype = ctypes.c_int
+    L.ms_device.argtypes = [vp, ctypes.POINTER(ctypes.c_int)]
     if path is None:
         _lib = L
     return L

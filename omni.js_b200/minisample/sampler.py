@@ -41,6 +41,17 @@ def _is_torch(x) -> bool:
     return type(x).__module__.startswith("torch")
 
 
+_SCORING = None
+
+
+def _scoring():
+    """The scoring module, which needs torch: loaded by the first call."""
+    global _SCORING
+    if _SCORING is None:
+        from . import scoring as _SCORING
+    return _SCORING
+
+
 class Sampler:
     """A libminisample context on one or more CUDA devices (the 'cuda' sampler backend)."""
 
@@ -55,6 +66,9 @@ class Sampler:
         if rc != N.MS_OK:
             raise N.MiniSampleError(rc, "ms_create failed (no CUDA device?)")
         self.devices = list(devices) if devices else None
+        d = ctypes.c_int()
+        self._L.ms_device(self._ctx, ctypes.byref(d))
+        self.device_index = d.value  # the CUDA device of device-pointer calls
 
     def close(self):
         if self._ctx:
@@ -119,6 +133,52 @@ class Sampler:
         n = ctypes.c_int64()
         self._check(self._L.ms_launch_count(self._ctx, ctypes.byref(n)))
         return n.value
+
+    # ------------------------------------------------------------------ scoring
+    def logprobs(self, logits, tokens=None, *, temperature=1.0, top_n=0, entropy=False, stats=False, stream=None):
+        """Log-probabilities under softmax(logits / temperature) of a [B, V]
+        float32, bfloat16 or float16 CUDA tensor, as a scoring.LogProbs:
+          logprobs      of `tokens`, int32 [B] or [B, n] (n <= 256), in that shape
+          entropy       [B] when `entropy`
+          top_ids, top_logprobs  [B, top_n] (top_n <= 256): the largest logits,
+                        equal ones by ascending id
+          row_max, row_sum  [B] when `stats`: what logprobs_backward takes
+        An id outside [0, V) is no token (log-probability 0); a row with no
+        token at all is padding (outputs 0, ids -1).  Differentiable: with
+        logits.requires_grad, logprobs and entropy carry gradients (top_ids and
+        top_logprobs do not).  Asynchronous, on `stream` or the current stream
+        (ms_logprobs)."""
+        return _scoring().logprobs(self, logits, tokens, temperature=temperature, top_n=top_n, entropy=entropy,
+                                   stats=stats, stream=stream)
+
+    def logprobs_backward(self, logits, tokens, row_max, row_sum, g_logprobs=None, g_entropy=None, entropy=None, *,
+                          temperature=1.0, out=None, stream=None):
+        """Gradient of the logits from the gradients g_logprobs (float32, the
+        tokens' shape) and g_entropy (float32 [B], with `entropy`), given what
+        logprobs(..., stats=True) returned for the same logits, tokens and
+        temperature.  `out` receives it (the logits themselves are allowed);
+        ms_logprobs_backward."""
+        return _scoring().logprobs_backward(self, logits, tokens, row_max, row_sum, g_logprobs, g_entropy, entropy,
+                                            temperature=temperature, out=out, stream=stream)
+
+    def distill_loss(self, logits, teacher_ids, teacher_values, *, temperature=1.0, kind="logprobs", stream=None):
+        """Divergence [B] of softmax(logits / temperature) from a teacher's top
+        ids (int32 [B, K], K <= 256, -1 where absent) and values (float32
+        [B, K]): kind "logprobs", log-probabilities at this temperature, whose
+        missing mass is held against the ids not listed; or "logits", softmaxed
+        over the list at this temperature.  Differentiable in the logits; a
+        training step that knows its row weights beforehand gets loss and
+        gradient from one pass with distill_grad (ms_distill)."""
+        return _scoring().distill_loss(self, logits, teacher_ids, teacher_values, temperature=temperature, kind=kind,
+                                       stream=stream)
+
+    def distill_grad(self, logits, teacher_ids, teacher_values, weight=None, *, temperature=1.0, kind="logprobs",
+                     out=None, stream=None):
+        """(loss [B], dlogits [B, V]): distill_loss and the gradient of
+        sum(weight * loss), weight float32 [B] (None: ones).  `out` receives the
+        gradient (the logits themselves are allowed); ms_distill."""
+        return _scoring().distill_grad(self, logits, teacher_ids, teacher_values, weight, temperature=temperature,
+                                       kind=kind, out=out, stream=stream)
 
     # ------------------------------------------------------------------ host
     def _sample_host(self, logits, params, u, hist, hist_off, diag, cand_cap, row_sharded, out, profile=False):
