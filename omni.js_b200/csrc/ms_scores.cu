@@ -10,21 +10,40 @@
 // alternatives.  Each thread keeps its own running maximum and fp32 sums of at
 // most a few hundred terms; threads are combined in fp64.
 //
+// A row is one thread-block cluster's: its CTAs take equal slices and exchange
+// their sums (a few numbers) through distributed shared memory, so a call needs
+// no scratch in global memory and one launch, whether it holds one row or
+// thousands.  The grid holds as many clusters as the GPU runs at once, each
+// working through its rows; every thread keeps a ring of asynchronous copies of
+// its own vectors in flight (shared memory that no other thread touches, so no
+// barrier guards it), which runs ahead into the next row while a row is
+// finished.  The reads of HBM bound the large calls, latency the small ones.
+//
 // A row's special cases follow from the same sums: a NaN or +Inf logit makes s
 // NaN (Inf - Inf), a row of -Inf alone leaves s = 0.
+#include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <mutex>
+#include <type_traits>
+#include <vector>
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "ms_scores.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace ms {
 namespace {
 
-constexpr int kRowThreads = 512;
-constexpr int kBuf = 1024;  // keys the selection holds: top_n (<= 256) and at least one tile of kRowThreads
+constexpr int kRowThreads = 256;
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kBatch = 4;       // 16-byte vectors of a thread's step
+constexpr int kMaxCluster = 16;
+constexpr int kBuf = 1024;      // keys the selection holds: top_n (<= 256) and at least one tile of kRowThreads
 
 // ---------------------------------------------------------------- row access
 // A row is read in 16-byte vectors on 16-byte boundaries, whatever its start:
@@ -128,80 +147,380 @@ __device__ __forceinline__ void store_vec(const Row<T>& R, T* d, bool same, int 
 }
 
 // ---------------------------------------------------------------- running sums
-// Sums over some of a row's elements, relative to their maximum m (-Inf and
-// s = 0 while there is none): s = sum 2^((x - m) a), q = sum 2^((x - m) a) (x - m).
+// Sums over some of a thread's elements: their maximum m (-Inf while there is
+// none), z = fp32(m a), and with y = x a - z, one rounding each,
+// s = sum 2^y and q = sum 2^y y, in two halves (the lanes of the paired fp32
+// instructions).  What z's rounding leaves, z - m a, is put right in fp64 when
+// the threads' sums are joined.  Where m a is beyond fp32 (|m| > 2e38: a row of
+// nothing but a type's lowest value, an Inf), y = (x - m) a instead.
+typedef unsigned long long f32x2;
 struct Sums {
-  float m = -INFINITY, s = 0.f, q = 0.f;
+  float m = -INFINITY, z = 0.f;
+  f32x2 s = 0, q = 0;
 };
 
-// x - m, bounded below so that a term of 0 times it is 0 (a NaN stays one)
-__device__ __forceinline__ float below(float x, float m) {
+// y, bounded below so that a term of 0 times it is 0 (a NaN stays one)
+__device__ __forceinline__ float bounded(float d) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d), "f"(-1e30f));
+  return r;
+}
+__device__ __forceinline__ float below(float x, float m) { return bounded(__fsub_rn(x, m)); }
+__device__ __forceinline__ f32x2 f2_mul(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float warp_max_f(float v) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(__fsub_rn(x, m)), "f"(-1e30f));
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
   return d;
 }
 
-template <int N, bool ENT>
-__device__ __forceinline__ void add_terms(Sums& t, const float (&f)[N], float a) {
-  float bm = f[0];
-#pragma unroll
-  for (int i = 1; i < N; i++) bm = fmaxf(bm, f[i]);
-  if (bm > t.m) {
-    const float d = below(t.m, bm);  // -1e30 for the first terms: the factor is 0
-    const float c = ex2_approx(d * a);
-    if constexpr (ENT) t.q = c * fmaf(t.s, d, t.q);
-    t.s *= c;
-    t.m = bm;
-  }
-  // while every element so far is -Inf any finite reference gives terms of 0
-  const float m = t.m == -INFINITY ? 0.f : t.m;
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    const float d = below(f[i], m);
-    const float e = ex2_approx(d * a);
-    t.s += e;
-    if constexpr (ENT) t.q = fmaf(e, d, t.q);
-  }
+// The step from a reference (m, z) to (M, Z), M >= m, in units of y.
+__device__ __forceinline__ float step_of(float m, float z, float M, float Z, float a) {
+  if (m == -INFINITY) return 0.f;  // sums of nothing (0), or of NaN alone: both stay
+  return bounded(isinf(Z) || isinf(z) ? __fsub_rn(m, M) * a : __fsub_rn(z, Z));
 }
 
-// The sums of a whole row, in fp64: relative to the row's maximum m.
+// A word of a vector as two fp32 elements (of 4-byte types: two words).
+__device__ __forceinline__ f32x2 pair_of(uint32_t a, uint32_t, __nv_bfloat16) {
+  return f2_pack(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+}
+__device__ __forceinline__ f32x2 pair_of(uint32_t a, uint32_t, __half) {
+  const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  return f2_pack(t.x, t.y);
+}
+__device__ __forceinline__ f32x2 pair_of(uint32_t a, uint32_t b, float) {
+  return f2_pack(__uint_as_float(a), __uint_as_float(b));
+}
+// The largest element of N words (a NaN is in no maximum).
+template <int N>
+__device__ __forceinline__ float largest(const uint32_t (&w)[N], __nv_bfloat16) {
+  __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
+#pragma unroll
+  for (int i = 1; i < N; i++) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+template <int N>
+__device__ __forceinline__ float largest(const uint32_t (&w)[N], __half) {
+  __half2 m = *reinterpret_cast<const __half2*>(&w[0]);
+#pragma unroll
+  for (int i = 1; i < N; i++) m = __hmax2(m, *reinterpret_cast<const __half2*>(&w[i]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+template <int N>
+__device__ __forceinline__ float largest(const uint32_t (&w)[N], float) {
+  float m = __uint_as_float(w[0]);
+#pragma unroll
+  for (int i = 1; i + 1 < N; i += 2) m = fmax3(m, __uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+  return fmaxf(m, __uint_as_float(w[N - 1]));
+}
+
+// A larger maximum: the sums carried over to it.
+template <bool ENT>
+__device__ __forceinline__ void raise_to(Sums& t, float hi, float a) {
+  const float z = hi * a, d = step_of(t.m, t.z, hi, z, a), c = ex2_approx(d);
+  const f32x2 c2 = f2_pack(c, c);
+  if constexpr (ENT) t.q = f2_mul(c2, f2_fma(t.s, f2_pack(d, d), t.q));
+  t.s = f2_mul(t.s, c2);
+  t.m = hi;
+  t.z = z;
+}
+
+// The terms of N words (N even), their maximum being in t.m already.
+template <typename T, int N, bool ENT>
+__device__ __forceinline__ void add_words(Sums& t, const uint32_t (&w)[N], float a) {
+  constexpr int PER = sizeof(T) == 4 ? 2 : 1;  // words a pair
+  const float hi = largest(w, T());
+  if (hi > t.m) raise_to<ENT>(t, hi, a);
+  const f32x2 z2 = f2_pack(-t.z, -t.z), a2 = f2_pack(a, a);
+  f32x2 s = t.s, q = t.q;
+#pragma unroll
+  for (int i = 0; i < N; i += PER) {
+    const f32x2 y2 = f2_fma(pair_of(w[i], w[i + PER - 1], T()), a2, z2);
+    const float2 y = f2_unpack(y2);
+    const f32x2 e = f2_pack(ex2_approx(y.x), ex2_approx(y.y));
+    s = f2_add(s, e);
+    if constexpr (ENT) q = f2_fma(e, y2, q);
+  }
+  // 0 times the y of a masked element, or an m a beyond fp32: once more, with care
+  bool odd = isinf(t.z);
+  if constexpr (ENT) {
+    const float2 h = f2_unpack(q);
+    odd |= isnan(h.x + h.y);
+  }
+  if (odd) {
+    const float m = t.m == -INFINITY ? 0.f : t.m;
+    s = t.s;
+    q = t.q;
+#pragma unroll
+    for (int i = 0; i < N; i += PER) {
+      const float2 x = f2_unpack(pair_of(w[i], w[i + PER - 1], T()));
+      const float y0 = bounded(isinf(t.z) ? __fsub_rn(x.x, m) * a : fmaf(x.x, a, -t.z));
+      const float y1 = bounded(isinf(t.z) ? __fsub_rn(x.y, m) * a : fmaf(x.y, a, -t.z));
+      const f32x2 e = f2_pack(ex2_approx(y0), ex2_approx(y1));
+      s = f2_add(s, e);
+      if constexpr (ENT) q = f2_fma(e, f2_pack(y0, y1), q);
+    }
+  }
+  t.s = s;
+  t.q = q;
+}
+
+template <bool ENT>
+__device__ __forceinline__ void add_term(Sums& t, float x, float a) {
+  const uint32_t w[2] = {__float_as_uint(x), 0xff800000u};
+  add_words<float, 2, ENT>(t, w, a);
+}
+
+// A warp's sums: {m, z, s, q} in every lane.
+template <bool ENT>
+__device__ __forceinline__ float4 warp_sums(const Sums& t, float a) {
+  const float m = warp_max_f(t.m), z = m == -INFINITY ? 0.f : m * a;
+  const float d = step_of(t.m, t.z, m, z, a), c = ex2_approx(d);
+  const float2 s2 = f2_unpack(t.s), q2 = f2_unpack(t.q);
+  float s = s2.x + s2.y, q = q2.x + q2.y;
+  q = c * fmaf(s, d, q);
+  s *= c;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    if constexpr (ENT) q += __shfl_xor_sync(0xffffffffu, q, o);
+  }
+  return make_float4(m, z, s, q);
+}
+
+// Sums of a CTA's or a row's elements in fp64: s = sum exp((x - m) / T) and
+// q = sum exp((x - m) / T) (x - m) / T for their maximum m.
 struct RowSums {
   float m;
   double s, q;
 };
 
-struct BlockScratch {
-  float m[32];
-  double s[32], q[32];
-};
+// exp(d), |d| next to 0 as a rule
+__device__ __forceinline__ double exp_small(double d) {
+  return fabs(d) < 1e-3 ? 1.0 + d * (1.0 + d * (0.5 + d * (1.0 / 6))) : exp(d);
+}
 
-__device__ __forceinline__ RowSums block_sums(const Sums& t, float a, BlockScratch& sh) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  const float wm = warp_max(t.m);
-  if (lane == 0) sh.m[warp] = wm;
-  __syncthreads();
-  RowSums r;
-  r.m = sh.m[0];
-  for (int w = 1; w < nw; w++) r.m = fmaxf(r.m, sh.m[w]);
-  // a thread without a finite or infinite element has s = 0 or NaN: both stay
-  const float d = t.m == -INFINITY ? 0.f : below(t.m, r.m);
-  const float c = ex2_approx(d * a);
-  double s = (double)t.s * c;
-  double q = ((double)t.q + (double)t.s * d) * c;
-  s = warp_sum(s);
-  q = warp_sum(q);
-  if (lane == 0) {
-    sh.s[warp] = s;
-    sh.q[warp] = q;
-  }
-  __syncthreads();
-  r.s = 0.0;
-  r.q = 0.0;
-  for (int w = 0; w < nw; w++) {
-    r.s += sh.s[w];
-    r.q += sh.q[w];
+// A warp's sums, relative to m itself.
+__device__ __forceinline__ RowSums exact_sums(float4 w, float a) {
+  const double ln2 = 0.693147180559945309417;
+  RowSums r = {w.x, (double)w.z, (double)w.w * ln2};
+  if (w.x != -INFINITY && !isinf(w.y)) {
+    const double d = ((double)w.y - (double)w.x * (double)a) * ln2;  // |d| <= |z| 2^-24
+    const double c = exp_small(d);
+    r.q = (r.q + r.s * d) * c;
+    r.s *= c;
   }
   return r;
+}
+
+// The sums of lanes 0 to 15's parts (m = -Inf, s = q = 0 for none) in every lane.
+template <bool ENT>
+__device__ __forceinline__ RowSums lane_sums(const RowSums& p, float a) {
+  RowSums r;
+  r.m = warp_max_f(p.m);
+  const float d = p.m == -INFINITY ? 0.f : below(p.m, r.m) * a;
+  const double c = (double)ex2_approx(d);
+  r.q = (p.q + p.s * (double)d * 0.693147180559945309417) * c;
+  r.s = p.s * c;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+    if constexpr (ENT) r.q += __shfl_xor_sync(0xffffffffu, r.q, o);
+  }
+  r.s = __shfl_sync(0xffffffffu, r.s, 0);
+  if constexpr (ENT) r.q = __shfl_sync(0xffffffffu, r.q, 0);
+  return r;
+}
+
+// The sums of the CTA's warps, from w[kRowWarps] in shared memory.
+template <bool ENT>
+__device__ __forceinline__ RowSums join_warps(const float4* w, float a) {
+  const int lane = threadIdx.x & 31;
+  return lane_sums<ENT>(lane < kRowWarps ? exact_sums(w[lane], a) : RowSums{-INFINITY, 0.0, 0.0}, a);
+}
+
+// Named barriers: the warps that only tell others something do not wait.
+__device__ __forceinline__ void bar_arrive(int id) { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "n"(kRowThreads) : "memory"); }
+__device__ __forceinline__ void bar_sync(int id) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "n"(kRowThreads) : "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// The CTA's slice of a row: whole vectors [w0, w1), thread t's being w0 + t,
+// w0 + t + kRowThreads, ..., kBatch of them a step; and the elements of a vector
+// that reaches over the row's first or last element, one a thread (`edge`, -1
+// for most threads).
+template <typename T>
+struct Slice {
+  static constexpr int VEC = Row<T>::VEC;
+  int w0, w1, edge;
+  __device__ __forceinline__ Slice(const Row<T>& R, int rank, int ranks) {
+    const int per = (R.nvec + ranks - 1) / ranks;
+    const int v0 = min(R.nvec, rank * per), v1 = min(R.nvec, v0 + per);
+    w0 = v0 + (v0 < v1 && !R.whole(v0));
+    w1 = v1 - (v1 > w0 && !R.whole(v1 - 1));
+    const int t = threadIdx.x;
+    edge = -1;
+    if (t < VEC && v0 < w0) edge = v0 * VEC - R.mis + t;
+    if (t >= VEC && t < 2 * VEC && w1 < v1) edge = w1 * VEC - R.mis + t - VEC;
+    if (edge >= R.V) edge = -1;
+  }
+  __device__ __forceinline__ int steps() const { return (w1 - w0 + kBatch * kRowThreads - 1) / (kBatch * kRowThreads); }
+  // vectors that this thread has in the last step (kBatch or fewer; less than 1 for none)
+  __device__ __forceinline__ int last() const {
+    return (w1 - w0 - (steps() - 1) * kBatch * kRowThreads - (int)threadIdx.x + kRowThreads - 1) / kRowThreads;
+  }
+  // the thread that holds element i, or -1 when it is not the slice's
+  __device__ __forceinline__ int owner(const Row<T>& R, int i, int rank, int ranks) const {
+    const int v = (i + R.mis) / VEC, l = (i + R.mis) % VEC;
+    if (v >= w0 && v < w1) return (v - w0) % kRowThreads;
+    const int per = (R.nvec + ranks - 1) / ranks;
+    if (v < rank * per || v >= min(R.nvec, (rank + 1) * per)) return -1;
+    return v < w0 ? l : VEC + l;
+  }
+};
+
+// ---------------------------------------------------------------- the ring
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most n of the thread's latest groups are in flight.
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int MOST>
+__device__ __forceinline__ void copies_wait(int n) {
+  if constexpr (MOST > 0) {
+    if (n >= MOST) copies_wait<MOST>();
+    else copies_wait<MOST - 1>(n);
+  } else {
+    copies_wait<0>();
+  }
+}
+
+// The rows first, first + step, ... that a cluster works on, and which of them
+// are read at all: those with an id inside [0, V) in their list of n (every row
+// when n = 0), and, where `weight` is given, a weight other than 0.  The row
+// after the one in question is looked up early (lane l holds entry l).
+struct RowList {
+  const int32_t* ids;
+  const float* weight;
+  int n, V;
+  int64_t B, step;
+  int pre;
+  float pre_w;
+  __device__ __forceinline__ void fetch(int64_t row) {
+    const int lane = threadIdx.x & 31;
+    pre = -1;
+    pre_w = 1.f;
+    if (row < B) {
+      if (lane < n) pre = ids[row * n + lane];
+      if (weight) pre_w = weight[row];
+    }
+  }
+  // for the row that was fetched last; the same in every thread of the cluster
+  __device__ __forceinline__ bool read(int64_t row) const {
+    if (n == 0) return true;
+    bool any = __any_sync(0xffffffffu, (uint32_t)pre < (uint32_t)V);
+    for (int j = 32 + (threadIdx.x & 31); !any && j - (int)(threadIdx.x & 31) < n; j += 32)
+      any = __any_sync(0xffffffffu, j < n && (uint32_t)ids[row * n + min(j, n - 1)] < (uint32_t)V);
+    return any && pre_w != 0.f;
+  }
+};
+
+// The copies of a thread's vectors, in the order of the rows and of their
+// steps, one group a step (an empty one when the rows are through).
+template <typename T, int DEPTH>
+struct Feed {
+  RowList rows;
+  const void* x;
+  int64_t ld, row;
+  int rank, ranks, left, last, slot;
+  const uint4* src;   // the thread's next vector
+  uint32_t ring;      // the thread's first place in shared memory
+  __device__ __forceinline__ void start(int64_t first) {
+    row = first;
+    slot = 0;
+    left = 0;
+    rows.fetch(row);
+    settle();
+#pragma unroll 1
+    for (int i = 0; i < DEPTH; i++) next();
+  }
+  // the next row, from `row` on, that is read and has vectors here
+  __device__ __forceinline__ void settle() {
+    while (row < rows.B) {
+      const bool yes = rows.read(row);
+      rows.fetch(row + rows.step);
+      if (yes) {
+        const Row<T> R(x, row, ld, rows.V);
+        const Slice<T> S(R, rank, ranks);
+        src = reinterpret_cast<const uint4*>(R.p - R.mis) + S.w0 + threadIdx.x;
+        left = S.steps();
+        last = S.last();
+        if (left > 0) return;
+      }
+      row += rows.step;
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if (left > 0) {
+      const uint32_t dst = ring + slot * (kBatch * kRowThreads * 16);
+      if (left > 1) {
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) copy16(dst + i * (kRowThreads * 16), src + i * kRowThreads);
+        src += kBatch * kRowThreads;
+        left--;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kBatch; i++)
+          if (i < last) copy16(dst + i * (kRowThreads * 16), src + i * kRowThreads);
+        left = 0;
+        row += rows.step;
+        settle();
+      }
+    }
+    slot = slot + 1 == DEPTH ? 0 : slot + 1;
+    copies_end_group();
+  }
+};
+
+// The words of a step's vectors out of the ring, those beyond the first n
+// vectors being elements of -Inf.
+template <typename T>
+__device__ __forceinline__ void ring_step(const uint4* src, int n, uint32_t (&w)[4 * kBatch]) {
+  constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+  for (int i = 0; i < kBatch; i++) {
+    uint4 u = make_uint4(none, none, none, none);
+    if (i < n) u = src[i * kRowThreads];
+    w[4 * i] = u.x;
+    w[4 * i + 1] = u.y;
+    w[4 * i + 2] = u.z;
+    w[4 * i + 3] = u.w;
+  }
+}
+
+// Element l of a thread's step (its vectors lie kRowThreads vectors apart, l
+// counting elements of memory from the first one) set to -Inf.
+template <typename T>
+__device__ __forceinline__ void mask_element(uint32_t (&w)[4 * kBatch], int l) {
+  constexpr int VEC = Row<T>::VEC, PER = VEC / 4;
+#pragma unroll
+  for (int i = 0; i < 4 * kBatch; i++) {
+    const int at = (i / 4) * (kRowThreads * VEC) + (i % 4) * PER;  // the word's first element
+    if constexpr (PER == 1) {
+      if (l == at) w[i] = 0xff800000u;
+    } else {
+      const uint32_t inf = std::is_same_v<T, __half> ? 0xfc00u : 0xff80u;
+      if (l == at) w[i] = (w[i] & 0xffff0000u) | inf;
+      if (l == at + 1) w[i] = (w[i] & 0xffffu) | (inf << 16);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- top alternatives
@@ -228,10 +547,73 @@ __device__ __forceinline__ void sort_desc(unsigned long long* k, int n) {
   __syncthreads();
 }
 
+constexpr int kRank = 512;  // keys up to which counting the larger ones is faster than sorting
+
 struct TopSmem {
   unsigned long long key[kBuf];
   int n;
 };
+
+constexpr int kRounds = kScoreMax / kRowWarps;  // bounds that a CTA gives for the largest top_n
+
+// A warp's share of the bounds for the alternatives: its j-th largest thread
+// maximum into red[j], j < rounds (-Inf where it has fewer).  The least of them
+// over the warps is reached by (j + 1) * kRowWarps of the CTA's elements at
+// least.  tm: the thread's largest element.
+__device__ __forceinline__ void top_maxima(float tm, int rounds, float (*red)[kRowWarps]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t key = fkey(tm);
+  for (int j = 0; j < rounds; j++) {
+    const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+    const unsigned who = __ballot_sync(0xffffffffu, key == best);
+    if (lane == __ffs(who) - 1) key = 0;  // one at a time: equal maxima count each
+    if (lane == 0) red[j][warp] = best <= fkey(-INFINITY) ? -INFINITY : fkey_inv(best);
+  }
+}
+
+// The row's bound from its CTAs' (each a list of `told`, largest first, in
+// `lists` one after the other): every bound at or above the rounds-th largest
+// of all of them stands for kRowWarps more elements.
+__device__ __forceinline__ float row_bound(const float* lists, int ranks, int told, int rounds) {
+  const int lane = threadIdx.x & 31;
+  int at = 0;
+  uint32_t best = 0;
+  for (int j = 0; j < rounds; j++) {
+    const uint32_t key = lane < ranks && at < told ? fkey(lists[lane * told + at]) : 0;
+    best = __reduce_max_sync(0xffffffffu, key);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, key == best)) - 1) at++;
+  }
+  return best <= fkey(-INFINITY) ? -INFINITY : fkey_inv(best);
+}
+
+// The CTA's elements >= bound, as keys into the buffer `to` (a peer's): only
+// threads whose maximum reaches the bound hold any, and the warp reads each
+// such thread's vectors again together.  Keys beyond the buffer are counted
+// and left out.  xe: the thread's edge element.
+template <typename T>
+__device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, float tm, float xe, float bound,
+                                           TopSmem* to) {
+  constexpr int VEC = Row<T>::VEC;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto take = [&](float x, int i) {
+    if (x >= bound && x > -INFINITY) {
+      const int n = atomicAdd(&to->n, 1);
+      if (n < kBuf) to->key[n] = top_key(x, i);
+    }
+  };
+  if (S.edge >= 0) take(xe, S.edge);
+  unsigned who = __ballot_sync(0xffffffffu, tm >= bound && tm > -INFINITY);
+  while (who) {
+    const int owner = warp * 32 + __ffs(who) - 1;
+    who &= who - 1;
+    for (int v = S.w0 + owner + lane * kRowThreads; v < S.w1; v += 32 * kRowThreads) {
+      float f[VEC];
+      load_vec(R, v, f);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) take(f[j], v * VEC - R.mis + j);
+    }
+  }
+}
 
 // The row's top_n keys, largest first, at the front of sh.key (0 beyond the
 // row's finite elements).  One element a thread at a time goes in when it
@@ -276,66 +658,236 @@ __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
 }
 
 // ---------------------------------------------------------------- forward
-// Whether a row counts: no tokens asked for, or one of its ids inside [0, V).
-__device__ __forceinline__ bool row_live(const ScoreArgs& A, int64_t r) {
-  if (A.n_tok == 0) return true;
-  int any = 0;
-  for (int t = threadIdx.x; t < A.n_tok; t += blockDim.x) any |= (uint32_t)A.tokens[r * A.n_tok + t] < (uint32_t)A.V;
-  return __syncthreads_or(any) != 0;
+// 3 CTAs an SM: their rings hold 192 KiB in flight.
+constexpr int kScoreCtas = 3, kScoreDepth = 4;
+constexpr int kScoreRing = kScoreDepth * kBatch * kRowThreads * 16;
+
+// A row's sums while they are joined, for a row and the next: the warps', and
+// the CTAs' (in the CTA that finishes the row).
+struct ScoreJoin {
+  float4 warp[2][kRowWarps];
+  RowSums cta[2][kMaxCluster];
+};
+struct TopJoin {
+  float bound[2][kRounds];              // what the CTA tells the others
+  union {
+    float red[kRounds][kRowWarps];      // before the CTAs meet
+    float lists[kRowThreads];           // what they all told, after it
+  };
+  TopSmem sel;                          // rank 0's is the row's
+};
+
+// A padded row's outputs, by one warp.
+__device__ __forceinline__ void write_padding(const ScoreArgs& A, int64_t r) {
+  const ms_scores& O = A.out;
+  const int lane = threadIdx.x & 31;
+  for (int t = lane; t < A.n_tok; t += 32)
+    if (O.logprobs) O.logprobs[r * A.n_tok + t] = 0.f;
+  for (int i = lane; i < A.top_n; i += 32) {
+    if (O.top_ids) O.top_ids[r * A.top_n + i] = -1;
+    if (O.top_logprobs) O.top_logprobs[r * A.top_n + i] = -INFINITY;
+  }
+  if (lane == 0) {
+    if (O.entropy) O.entropy[r] = 0.f;
+    if (O.row_max) O.row_max[r] = 0.0;
+    if (O.row_sum) O.row_sum[r] = 0.0;
+  }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) logprobs_kernel(ScoreArgs A) {
-  __shared__ BlockScratch bs;
-  __shared__ TopSmem top;
-  constexpr int VEC = Row<T>::VEC;
-  const int64_t r = blockIdx.x;
-  const Row<T> R(A.x, r, A.ld, A.V);
-  const int32_t* tok = A.tokens + r * A.n_tok;
+// log s for s >= 1, in fp32's precision near 1 too
+__device__ __forceinline__ double log_sum(double s) {
+  if (s < 1.0) s = 1.0;  // the largest term is 1 but for its rounding
+  return s < 2.0 ? (double)log1pf((float)(s - 1.0)) : (double)logf((float)s);
+}
+
+// A row's numbers and its tokens' log-probabilities from its sums, by one warp.
+// log s is -Inf for a row of -Inf alone, NaN for a NaN row.
+template <typename T, bool ENT>
+__device__ __forceinline__ void write_row(const ScoreArgs& A, int64_t r, const Row<T>& R, const RowSums& sum) {
   const ms_scores& O = A.out;
-  if (!row_live(A, r)) {
-    for (int t = threadIdx.x; t < A.n_tok; t += blockDim.x)
-      if (O.logprobs) O.logprobs[r * A.n_tok + t] = 0.f;
-    for (int i = threadIdx.x; i < A.top_n; i += blockDim.x) {
-      if (O.top_ids) O.top_ids[r * A.top_n + i] = -1;
-      if (O.top_logprobs) O.top_logprobs[r * A.top_n + i] = -INFINITY;
-    }
-    if (threadIdx.x == 0) {
-      if (O.entropy) O.entropy[r] = 0.f;
-      if (O.row_max) O.row_max[r] = 0.0;
-      if (O.row_sum) O.row_sum[r] = 0.0;
-    }
-    return;
-  }
-  Sums t;
-  for (int v = threadIdx.x; v < R.nvec; v += blockDim.x) {
-    float f[VEC];
-    load_vec(R, v, f);
-    add_terms<VEC, true>(t, f, A.a);
-  }
-  const RowSums S = block_sums(t, A.a, bs);
-  const double log_s = log(S.s);  // -Inf for a row of -Inf alone, NaN for a NaN row
-  const bool empty = S.s == 0.0;
-  auto logprob = [&](float x) { return empty ? -INFINITY : (float)(((double)x - (double)S.m) / A.T - log_s); };
-  if (threadIdx.x == 0) {
-    if (O.entropy) O.entropy[r] = empty ? 0.f : (float)(log_s - S.q / S.s / A.T);
-    if (O.row_max) O.row_max[r] = (double)S.m / A.T;
-    if (O.row_sum) O.row_sum[r] = S.s;
-  }
+  const int lane = threadIdx.x & 31;
+  const double log_s = sum.s == 0.0 ? -INFINITY : log_sum(sum.s);
+  const bool empty = sum.s == 0.0;
   if (O.logprobs)
-    for (int i = threadIdx.x; i < A.n_tok; i += blockDim.x) {
-      const int y = tok[i];
-      O.logprobs[r * A.n_tok + i] = (uint32_t)y < (uint32_t)A.V ? logprob(to_f(R.p[y])) : 0.f;
+    for (int t = lane; t < A.n_tok; t += 32) {
+      const int y = A.tokens[r * A.n_tok + t];
+      float lp = 0.f;
+      if ((uint32_t)y < (uint32_t)A.V)
+        lp = empty ? -INFINITY : (float)(((double)to_f(R.p[y]) - (double)sum.m) * A.rT - log_s);
+      O.logprobs[r * A.n_tok + t] = lp;
     }
-  if (A.top_n == 0) return;
-  const bool bad = !(S.s >= 0.0);
-  if (!bad) top_scan(R, A.top_n, top);
-  for (int i = threadIdx.x; i < A.top_n; i += blockDim.x) {
-    const unsigned long long k = bad ? 0ull : top.key[i];
-    if (O.top_ids) O.top_ids[r * A.top_n + i] = k ? (int32_t)~(uint32_t)k : -1;
-    if (O.top_logprobs)
-      O.top_logprobs[r * A.top_n + i] = k ? logprob(fkey_inv((uint32_t)(k >> 32))) : (bad ? (float)S.s : -INFINITY);
+  if (lane == 0) {
+    if (ENT) O.entropy[r] = empty ? 0.f : (float)(log_s - sum.q / sum.s);
+    if (O.row_max) O.row_max[r] = (double)sum.m / A.T;
+    if (O.row_sum) O.row_sum[r] = sum.s;
   }
+}
+
+// A cluster's rows, one after the other.  Every warp sums its share of the
+// slice.  Without alternatives only the warp whose turn it is waits for the
+// others: it joins the CTA's sums and hands them to the CTA whose turn it is,
+// which writes the row; both turns go round, and everyone else is at the next
+// row meanwhile (the joins are double, and a warp is never two rows ahead: it
+// passes the cluster's barrier of the row before).
+//
+// With alternatives, every CTA also finds bounds that top_n of its elements
+// reach, from the thread maxima that the sums need anyway.  The best bound of
+// all the CTAs' is reached by top_n elements of the row, so the alternatives
+// are among the elements that reach it: about top_n and a few more, held by
+// about top_n threads, whose vectors (and no others) are read once more, out
+// of L2.  Rank 0 gathers and orders them.
+template <typename T, bool ENT, bool TOP>
+__global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(ScoreArgs A) {
+  extern __shared__ uint4 ring[];
+  __shared__ ScoreJoin join;
+  __shared__ std::conditional_t<TOP, TopJoin, int> top_smem;
+  TopJoin& tp = reinterpret_cast<TopJoin&>(top_smem);
+  TopSmem* const top = &tp.sel;
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank(), ranks = (int)cl.num_blocks();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // bounds that the alternatives need, and those that each CTA tells: twice its share and two more
+  const int rounds = (A.top_n + kRowWarps - 1) / kRowWarps;
+  const int told = ranks == 1 ? rounds : min(rounds, (2 * rounds + ranks - 1) / ranks + 2);
+  const int64_t first = blockIdx.x / ranks, step = gridDim.x / ranks;
+  const ms_scores& O = A.out;
+  Feed<T, kScoreDepth> feed;
+  feed.rows = {A.tokens, nullptr, A.n_tok, A.V, A.B, step, -1, 1.f};
+  RowList rows = feed.rows;  // the rows as they are worked on
+  feed.x = A.x;
+  feed.ld = A.ld;
+  feed.rank = rank;
+  feed.ranks = ranks;
+  feed.ring = smem_addr(ring + tid);
+  feed.start(first);
+  rows.fetch(first);
+  int slot = 0, which = 0, turn_rank = 0, turn_warp = 0;
+  cluster_arrive();
+  bool waiting = true;  // for the cluster's barrier of the row before (at first: for its CTAs to have started)
+  for (int64_t r = first; r < A.B; r += step) {
+    const bool live = rows.read(r);  // the same in every CTA of the cluster
+    rows.fetch(r + step);
+    if (!live) {
+      if (rank == 0 && warp == 0) write_padding(A, r);
+      continue;
+    }
+    const Row<T> R(A.x, r, A.ld, A.V);
+    const Slice<T> S(R, rank, ranks);
+    const float xe = S.edge >= 0 ? to_f(R.p[S.edge]) : -INFINITY;
+    if (TOP && tid == 0) top->n = 0;
+
+    Sums t;
+    const int steps = S.steps(), last = S.last();
+    for (int k = 1; k <= steps; k++) {
+      copies_wait<kScoreDepth - 1>();
+      uint32_t w[4 * kBatch];
+      ring_step<T>(ring + slot * (kBatch * kRowThreads) + tid, k < steps ? kBatch : last, w);
+      slot = slot + 1 == kScoreDepth ? 0 : slot + 1;
+      add_words<T, 4 * kBatch, ENT>(t, w, A.a);
+      feed.next();
+    }
+    if (S.edge >= 0) add_term<ENT>(t, xe, A.a);
+    const float4 ws = warp_sums<ENT>(t, A.a);
+    if (lane == 0) join.warp[which][warp] = ws;
+
+    if constexpr (!TOP) {
+      __syncwarp();
+      if (warp == turn_warp) {
+        bar_sync(1 + which);
+        const RowSums mine = join_warps<ENT>(join.warp[which], A.a);
+        if (waiting) cluster_wait();
+        if (ranks == 1) write_row<T, ENT>(A, r, R, mine);
+        else if (lane == 0) *cl.map_shared_rank(&join.cta[which][rank], turn_rank) = mine;
+        __syncwarp();
+      } else {
+        bar_arrive(1 + which);
+        if (waiting) cluster_wait();
+      }
+      cluster_arrive();
+      waiting = true;
+      if (ranks > 1 && rank == turn_rank && warp == turn_warp) {
+        cluster_wait();
+        waiting = false;
+        const RowSums sum = lane_sums<ENT>(lane < ranks ? join.cta[which][lane] : RowSums{-INFINITY, 0.0, 0.0}, A.a);
+        write_row<T, ENT>(A, r, R, sum);
+      }
+      which ^= 1;
+      if (++turn_rank == ranks) {
+        turn_rank = 0;
+        turn_warp = turn_warp + 1 == kRowWarps ? 0 : turn_warp + 1;
+      }
+    } else {
+      top_maxima(t.m, told, tp.red);
+      __syncthreads();
+      if (waiting) cluster_wait();
+      waiting = false;
+      if (warp == 0) {
+        const RowSums mine = join_warps<ENT>(join.warp[which], A.a);
+        if (lane < told) {
+          float b = tp.red[lane][0];
+#pragma unroll
+          for (int w = 1; w < kRowWarps; w++) b = fminf(b, tp.red[lane][w]);
+          tp.bound[which][lane] = b;
+        }
+        if (lane == 0) *cl.map_shared_rank(&join.cta[which][rank], 0) = mine;
+        __syncwarp();
+      }
+      cluster_arrive();
+      cluster_wait();
+      float bound = tp.bound[which][rounds - 1];
+      if (ranks > 1) {
+        if (tid < ranks * told) tp.lists[tid] = cl.map_shared_rank(tp.bound[which], tid / told)[tid % told];
+        __syncthreads();
+        bound = row_bound(tp.lists, ranks, told, rounds);
+      }
+      top_gather(R, S, t.m, xe, bound, cl.map_shared_rank(top, 0));
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();  // the gathered keys are rank 0's
+      const int now = which;
+      which ^= 1;
+      if (rank != 0) continue;
+      const RowSums sum = lane_sums<ENT>(lane < ranks ? join.cta[now][lane] : RowSums{-INFINITY, 0.0, 0.0}, A.a);
+      if (warp == kRowWarps - 1) write_row<T, ENT>(A, r, R, sum);
+      const double log_s = log_sum(sum.s);
+      auto logprob = [&](float x) { return (float)(((double)x - (double)sum.m) * A.rT - log_s); };
+      const bool bad = !(sum.s >= 0.0);
+      const int n = top->n;
+      auto put = [&](int i, unsigned long long k) {
+        if (O.top_ids) O.top_ids[r * A.top_n + i] = k ? (int32_t)~(uint32_t)k : -1;
+        if (O.top_logprobs)
+          O.top_logprobs[r * A.top_n + i] = k ? logprob(fkey_inv((uint32_t)(k >> 32))) : (bad ? (float)sum.s : -INFINITY);
+      };
+      if (bad) {
+        for (int i = tid; i < A.top_n; i += kRowThreads) put(i, 0);
+      } else if (n <= kRank) {
+        // a key's place is the number of larger ones
+        for (int i = tid; i < n; i += kRowThreads) {
+          const unsigned long long k = top->key[i];
+          int place = 0;
+#pragma unroll 8
+          for (int j = 0; j < n; j++) place += top->key[j] > k;
+          if (place < A.top_n) put(place, k);
+        }
+        for (int i = n + tid; i < A.top_n; i += kRowThreads) put(i, 0);
+      } else {
+        if (n <= kBuf) {
+          for (int i = n + tid; i < kBuf; i += kRowThreads) top->key[i] = 0;
+          sort_desc(top->key, kBuf);
+        } else {  // rows whose largest elements crowd into few threads, or tie by the hundred
+          __syncthreads();  // every thread has read n
+          top_scan(R, A.top_n, *top);
+        }
+        for (int i = tid; i < A.top_n; i += kRowThreads) put(i, top->key[i]);
+      }
+      __syncthreads();  // before the next row's keys
+    }
+  }
+  copies_wait<0>();
+  if (waiting) cluster_wait();
+  __syncwarp();
+  cluster_arrive();  // no CTA ends while a peer may write to it or read from it
+  cluster_wait();
 }
 
 // ---------------------------------------------------------------- backward
@@ -368,6 +920,14 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
     any |= ok;
   }
   const bool live = __syncthreads_or(any) != 0 || A.n_tok == 0;
+  // the thread's vectors are on their way while the row's numbers are read
+  const bool inner = live && v1 - v0 == kGradThreads * kGradVecs && R.whole(v0) && R.whole(v1 - 1);
+  uint4 u[kGradVecs];
+  if (inner) {
+    const uint4* p = reinterpret_cast<const uint4*>(R.p - R.mis) + v0 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kGradVecs; i++) u[i] = p[i * kGradThreads];
+  }
   const double S = live ? A.row_sum[r] : 0.0;
   double G = 0.0;
   for (int t = 0; t < A.n_tok; t++) G += (double)s_g[t];
@@ -381,20 +941,31 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
   const double k = -A.rT / S;
   const float c0 = (float)(k * (G + gH * (H - log_s)));
   const float c1 = (float)(k * gH * A.rT);
-  for (int v = v0 + threadIdx.x; v < v1; v += kGradThreads) {
-    float f[VEC];
-    if (zero) {
+  auto put = [&](int v, float(&f)[VEC]) {
 #pragma unroll
-      for (int j = 0; j < VEC; j++) f[j] = 0.f;
-    } else {
-      load_vec(R, v, f);
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        const float dd = below(f[j], m);
-        f[j] = ex2_approx(dd * A.a) * fmaf(c1, dd, c0);
-      }
+    for (int j = 0; j < VEC; j++) {
+      const float dd = below(f[j], m);
+      f[j] = ex2_approx(dd * A.a) * fmaf(c1, dd, c0);
     }
     store_vec(R, d, same, v, f);
+  };
+  const int v = v0 + threadIdx.x;
+  if (zero) {
+    const float f[VEC] = {};
+    for (int w = v; w < v1; w += kGradThreads) store_vec(R, d, same, w, f);
+  } else if (inner) {
+#pragma unroll
+    for (int i = 0; i < kGradVecs; i++) {
+      float f[VEC];
+      unpack(u[i], f, T());
+      put(v + i * kGradThreads, f);
+    }
+  } else {
+    for (int w = v; w < v1; w += kGradThreads) {
+      float f[VEC];
+      load_vec(R, w, f);
+      put(w, f);
+    }
   }
   if (!tokens_too) return;
   __syncthreads();
@@ -415,185 +986,427 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
 }
 
 // ---------------------------------------------------------------- distillation
-struct DistillSmem {
+// What is joined of a row: the sums of the ids not listed and of the listed
+// ones, the warps' and the CTA's (which the others of the cluster read).
+struct DistillJoin {
+  float4 warp[kRowWarps], warp_listed[kRowWarps];
+  RowSums others, listed;
+};
+// The teacher's list of a row, and what its warps add up of it: the masses,
+// relative to exp(m / T) for a list of logits, and the terms of the loss.
+struct DistillList {
   int id[kScoreMax];       // the listed ids, -1 where absent
-  float x[kScoreMax];      // their logits
   double q[kScoreMax];     // the teacher's masses
-  double red[32];
-  int first[kScoreMax];    // 1: the id's first place in the list
-  int next[kRowThreads];   // the first vector step of a thread that holds a listed id
+  int head[kRowThreads];   // the listed ids that a thread's vectors hold, as a chain of places in the list
+  int link[kScoreMax];
+  float m[kRowWarps];
+  double mass[kRowWarps], loss[kRowWarps];
 };
 
-// Sum of one value a thread, the same in every thread, in a fixed order.
-__device__ __forceinline__ double block_sum(double v, double* red) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double t = 0.0;
-  for (int w = 0; w < (int)(blockDim.x >> 5); w++) t += red[w];
-  return t;
-}
-__device__ __forceinline__ float block_max(float v, double* red) {
-  v = warp_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = (double)v;
-  __syncthreads();
-  float t = -INFINITY;
-  for (int w = 0; w < (int)(blockDim.x >> 5); w++) t = fmaxf(t, (float)red[w]);
-  return t;
-}
-
-// One row: the teacher's list (thread j holds entry j), then the row's sums
-// without the listed ids, so that the mass outside the list is a sum of its own
-// and no difference of two near 1, then the gradient over the row again.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) distill_kernel(DistillArgs A) {
-  __shared__ DistillSmem sh;
-  __shared__ BlockScratch bs;
-  constexpr int VEC = Row<T>::VEC;
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x, K = A.K;
-  const Row<T> R(A.x, r, A.ld, A.V);
-  T* d = (T*)A.dx + r * A.dld;
-  const bool same = (((uintptr_t)d ^ (uintptr_t)R.p) & 15) == 0;
+__device__ __forceinline__ void zero_slice(const Row<T>& R, const Slice<T>& S, T* d, bool same) {
+  const float f[Row<T>::VEC] = {};
+  for (int v = S.w0 + threadIdx.x; v < S.w1; v += kRowThreads) store_vec(R, d, same, v, f);
+  if (S.edge >= 0) d[S.edge] = from_f<T>(0.f);
+}
 
-  // ---- the teacher
-  int id = -1;
-  float val = -INFINITY;
-  if (tid < K) {
-    id = A.ids[r * K + tid];
-    val = A.values[r * K + tid];
-    // an id outside the vocabulary is absent, and so is a logit of -Inf
-    if ((uint32_t)id >= (uint32_t)A.V || (A.kind == MS_TEACHER_LOGITS && val == -INFINITY)) id = -1;
-    sh.id[tid] = id;
-  }
-  sh.next[tid] = INT_MAX;
-  const bool live = __syncthreads_or(id >= 0) != 0;
-  const float w = A.weight ? A.weight[r] : 1.f;
-  const bool grad = A.dx != nullptr && live && w != 0.f;
-  if (!live || (!grad && !A.loss)) {
-    if (tid == 0 && A.loss) A.loss[r] = 0.f;
-    if (A.dx) {
-      const float f[VEC] = {};
-      for (int v = tid; v < R.nvec; v += blockDim.x) store_vec(R, d, same, v, f);
+// 2 CTAs an SM; a slice of up to 96 KiB stays in its threads' rings.
+constexpr int kDistillCtas = 2, kDistillDepth = 6;
+constexpr int kDistillRing = kDistillDepth * kBatch * kRowThreads * 16;
+
+// A cluster's rows, one after the other.  The teacher's list (thread j holds
+// entry j) is every CTA's; the sums are over the ids that are not listed, so
+// that the mass outside the list is a sum of its own and no difference of two
+// near 1; the listed ids come out of the vectors as they are read, each thread
+// following the chain of those that its vectors hold.  The gradient is a
+// second pass over the slice: over the ring, which holds the whole slice (KEEP)
+// and takes in the next row's step for each one that is written, or out of L2
+// where a slice is larger.
+template <typename T, bool KEEP>
+__global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(DistillArgs A) {
+  static_assert(kScoreMax <= kRowThreads, "one list entry a thread");
+  extern __shared__ uint4 ring[];
+  __shared__ DistillList list[2];  // a row's and the next's
+  __shared__ DistillJoin join[2];
+  constexpr int VEC = Row<T>::VEC, STEP = kBatch * kRowThreads;
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank(), ranks = (int)cl.num_blocks();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = A.K;
+  const bool logits = A.kind == MS_TEACHER_LOGITS;
+  const int64_t begin = blockIdx.x / ranks, stride = gridDim.x / ranks;
+  Feed<T, kDistillDepth> feed;
+  feed.rows = {A.ids, A.loss ? nullptr : A.weight, K, A.V, A.B, stride, -1, 1.f};
+  feed.x = A.x;
+  feed.ld = A.ld;
+  feed.rank = rank;
+  feed.ranks = ranks;
+  feed.ring = smem_addr(ring + tid);
+  feed.start(begin);
+  int slot = 0, which = 0, joined = 0, turn = 0;
+  int id_in = -1;  // thread j's entry of the row after the next prepared one, and its weight
+  float val_in = -INFINITY, w_in = 1.f;
+  auto fetch = [&](int64_t r) {
+    if (r >= A.B) return;
+    if (tid < K) {
+      id_in = A.ids[r * K + tid];
+      val_in = A.values[r * K + tid];
     }
-    return;
-  }
-  double log_q = (double)val;
-  if (A.kind == MS_TEACHER_LOGITS) {
-    const float top = block_max(id >= 0 ? val : -INFINITY, sh.red);
-    const double dv = ((double)val - (double)top) / A.T;
-    log_q = dv - log(block_sum(id >= 0 ? exp(dv) : 0.0, sh.red));
-  }
-  const double q = id >= 0 ? exp(log_q) : 0.0;
-  const double Q = block_sum(q, sh.red);
-  double rest = A.kind == MS_TEACHER_LOGITS ? 0.0 : 1.0 - Q;
-  if (rest < kNoTail) rest = 0.0;
-  float xl = -INFINITY;
-  bool first = false;
-  if (id >= 0) {
-    xl = to_f(R.p[id]);
-    first = true;
-    for (int j = 0; j < tid; j++) first &= sh.id[j] != id;
-    const int v = (id + R.mis) / VEC;
-    atomicMin(&sh.next[v % kRowThreads], v / kRowThreads);
-  }
-  if (tid < K) {
-    sh.q[tid] = q;
-    sh.first[tid] = first;
-  }
-  __syncthreads();
+    if (A.weight) w_in = A.weight[r];
+  };
+  // The list of the row that was fetched, into L: the ids and their masses, by warp.
+  int id_next = -1;
+  float val_next = -INFINITY, w_next = 1.f;
+  auto prepare = [&](DistillList& L, int64_t after) {
+    id_next = (uint32_t)id_in < (uint32_t)A.V ? id_in : -1;  // absent outside the vocabulary
+    val_next = val_in;
+    w_next = w_in;
+    fetch(after);
+    L.head[tid] = -1;
+    if (warp * 32 >= K) {
+      id_next = -1;
+      if (lane == 0) L.m[warp] = -INFINITY, L.mass[warp] = 0.0;
+      return;
+    }
+    const int id = logits && val_next == -INFINITY ? -1 : id_next;  // a logit of -Inf is absent too
+    const float vm = logits ? warp_max_f(id >= 0 ? val_next : -INFINITY) : 0.f;
+    const double q = id < 0 ? 0.0 : exp(logits ? ((double)val_next - (double)vm) * A.rT : (double)val_next);
+    L.id[tid] = id;
+    L.q[tid] = q;
+    const double mass = warp_sum(q);
+    if (lane == 0) L.m[warp] = vm, L.mass[warp] = mass;
+  };
+  fetch(begin);
+  prepare(list[0], begin + stride);
+  for (int64_t r = begin; r < A.B; r += stride, which ^= 1) {
+    const Row<T> R(A.x, r, A.ld, A.V);
+    const Slice<T> S(R, rank, ranks);
+    T* d = (T*)A.dx + r * A.dld;
+    const bool same = (((uintptr_t)d ^ (uintptr_t)R.p) & 15) == 0;
+    const int steps = S.steps(), last = S.last();
+    DistillList& L = list[which];
+    DistillJoin& J = join[joined];
+    const float w = w_next, val = val_next;
+    const bool read = __syncthreads_or(id_next >= 0) != 0 && (A.loss || w != 0.f);  // as the feed has it
+    const bool grad = A.dx != nullptr && w != 0.f;
+    if (!read) {  // in every CTA of the cluster
+      if (tid == 0 && rank == 0 && A.loss) A.loss[r] = 0.f;
+      if (A.dx) zero_slice(R, S, d, same);
+      prepare(list[which ^ 1], r + 2 * stride);
+      continue;
+    }
+    joined ^= 1;  // with the cluster's barriers, which rows that are not read do not reach
 
-  // ---- the row's sums over the ids that are not listed
-  Sums t;
-  int next = sh.next[tid];
-  for (int v = tid, step = 0; v < R.nvec; v += kRowThreads, step++) {
-    float f[VEC];
-    load_vec(R, v, f);
-    if (step == next) {  // this vector holds a listed id: take them out, and find the thread's next
-      next = INT_MAX;
-      const int i0 = v * VEC - R.mis;
-      for (int j = 0; j < K; j++) {
-        const int i = sh.id[j];
-        if (i < 0) continue;
-        const int vj = (i + R.mis) / VEC;
-        if (vj == v) {
+    // ---- the list
+    const int id = warp * 32 < K ? L.id[tid] : -1;
+    const bool mine = rank == turn;  // this CTA writes the row's loss
+    if (++turn == ranks) turn = 0;
+    const int own = id >= 0 ? S.owner(R, id, rank, ranks) : -1;
+    const bool inside = own >= 0;
+    float xl = -INFINITY;
+    if (inside || (mine && id >= 0)) xl = to_f(R.p[id]);
+    if (inside) L.link[tid] = atomicExch(&L.head[own], tid);
+    const float xe = S.edge >= 0 ? to_f(R.p[S.edge]) : -INFINITY;
+    __syncthreads();
+
+    // ---- the sums over the ids that are not listed
+    Sums t;
+    const int head = L.head[tid];
+    // the thread's first vector at or after v that holds a listed id
+    auto next_from = [&](int v) {
+      int next = INT_MAX;
+      for (int j = head; j >= 0; j = L.link[j]) {
+        const int vj = (L.id[j] + R.mis) / VEC;
+        if (vj >= v && vj < S.w1) next = min(next, vj);
+      }
+      return next;
+    };
+    int next = next_from(S.w0);
+    const int slot0 = slot;
+    for (int k = 0, v = S.w0 + tid; k < steps; k++, v += STEP) {
+      // KEEP: no copies start in this pass, so fewer and fewer are in flight behind the step's
+      if (KEEP) copies_wait<kDistillDepth - 1>(kDistillDepth - 1 - k);
+      else copies_wait<kDistillDepth - 1>();
+      uint32_t x[4 * kBatch];
+      ring_step<T>(ring + slot * STEP + tid, k + 1 < steps ? kBatch : last, x);
+      slot = slot + 1 == kDistillDepth ? 0 : slot + 1;
+      if (next < v + STEP) {
+        for (int j = head; j >= 0; j = L.link[j]) mask_element<T>(x, L.id[j] + R.mis - v * VEC);
+        next = next_from(v + STEP);
+      }
+      add_words<T, 4 * kBatch, false>(t, x, A.a);
+      if (!KEEP) feed.next();
+    }
+    if (S.edge >= 0) {
+      bool listed = false;
+      for (int j = head; j >= 0; j = L.link[j]) listed |= L.id[j] == S.edge;
+      if (!listed) add_term<false>(t, xe, A.a);
+    }
+    const float4 ws = warp_sums<false>(t, A.a);
+    float4 wl = {-INFINITY, 0.f, 0.f, 0.f};
+    bool first = inside, twice = false;  // an id's first place in the list stands for it
+    if (warp * 32 < K) {
+      if (inside)
+        for (int j = L.head[own]; j >= 0; j = L.link[j])
+          if (j != tid && L.id[j] == id) {
+            twice = true;
+            first &= tid < j;
+          }
+      Sums tl;
+      if (first) add_term<false>(tl, xl, A.a);
+      wl = warp_sums<false>(tl, A.a);
+    }
+    if (lane == 0) {
+      J.warp[warp] = ws;
+      J.warp_listed[warp] = wl;
+    }
+    __syncthreads();
+
+    // ---- the row's sums
+    if (warp == 0) {
+      const RowSums o = join_warps<false>(J.warp, A.a), l = join_warps<false>(J.warp_listed, A.a);
+      if (lane == 0) {
+        J.others = o;
+        J.listed = l;
+      }
+      __syncwarp();
+    }
+    cluster_arrive();
+    prepare(list[which ^ 1], r + 2 * stride);  // meanwhile
+    double Q = 0.0, log_top = 0.0;  // the teacher's mass; for logits, its log relative to the largest
+    float top = 0.f;
+    bool live = true;               // some entry is present
+    if (logits) {
+      top = -INFINITY;
 #pragma unroll
-          for (int l = 0; l < VEC; l++)
-            if (i0 + l == i) f[l] = -INFINITY;
-        } else if (vj % kRowThreads == tid && vj > v) {
-          next = min(next, vj / kRowThreads);
+      for (int i = 0; i < kRowWarps; i++) top = fmaxf(top, L.m[i]);
+#pragma unroll
+      for (int i = 0; i < kRowWarps; i++)
+        if (L.mass[i] != 0.0) Q += L.mass[i] * exp(((double)L.m[i] - (double)top) * A.rT);
+      live = Q != 0.0;
+      log_top = log(Q);
+      Q = Q == Q ? 1.0 : Q;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRowWarps; i++) Q += L.mass[i];
+    }
+    double rest = logits ? 0.0 : 1.0 - Q;
+    if (rest < kNoTail) rest = 0.0;
+    const double wt = (double)w * A.rT, all = Q + rest;
+    // an entry's log mass, and its mass
+    auto log_q = [&] { return logits ? ((double)val - (double)top) * A.rT - log_top : (double)val; };
+    auto mass = [&] { return id < 0 ? 0.0 : logits ? exp(log_q()) : L.q[tid]; };
+    cluster_wait();
+    RowSums O = {-INFINITY, 0.0, 0.0}, l = O;
+    if (lane < ranks) {
+      const DistillJoin* p = cl.map_shared_rank(&J, lane);
+      O = p->others;
+      l = p->listed;
+    }
+    O = lane_sums<false>(O, A.a);
+    l = lane_sums<false>(l, A.a);
+    const float m = fmaxf(O.m, l.m);
+    // from the other ids' and the listed ones' maximum to the row's
+    const double scale = O.m == -INFINITY ? 1.0 : (double)ex2_approx(below(O.m, m) * A.a);
+    const double scale_l = l.m == -INFINITY ? 1.0 : (double)ex2_approx(below(l.m, m) * A.a);
+    const double s = O.s * scale + l.s * scale_l;
+    const bool empty = s == 0.0;
+    if (A.loss && mine) {
+      const double log_s = log(s);
+      double loss = 0.0;
+      if (warp * 32 < K) {
+        const double q = mass();
+        if (q != 0.0) loss = q * (log_q() - (((double)xl - (double)m) * A.rT - log_s));
+        loss = warp_sum(loss);
+      }
+      if (lane == 0) L.loss[warp] = loss;
+      __syncthreads();
+      if (tid == 0) {
+        loss = 0.0;
+        for (int i = 0; i < kRowWarps; i++) loss += L.loss[i];
+        if (rest != 0.0) {
+          const double gap = O.m == -INFINITY ? 0.0 : ((double)O.m - (double)m) * A.rT;
+          loss += rest * (log(rest) - (log(O.s) + gap - log_s));
         }
+        if (empty) loss = INFINITY;
+        A.loss[r] = live ? (float)loss : 0.f;
       }
     }
-    add_terms<VEC, false>(t, f, A.a);
-  }
-  const float ml = block_max(first ? xl : -INFINITY, sh.red);
-  RowSums S = block_sums(t, A.a, bs);
-  const float m = fmaxf(S.m, ml);
-  // a listed NaN is in no maximum; its term below makes the row NaN
-  const double gap = S.m == -INFINITY ? 0.0 : ((double)S.m - (double)m) / A.T;
-  const double scale = exp(gap);  // from the other ids' maximum to the row's
-  const double tail = S.s * scale;
-  const bool none = m == -INFINITY;
-  const double e = first ? (xl == -INFINITY ? 0.0 : exp(((double)xl - (none ? 0.0 : (double)m)) / A.T)) : 0.0;
-  const double s = tail + block_sum(e, sh.red);
-  const bool empty = s == 0.0;
-  const double log_s = log(s);
-  if (A.loss) {
-    double term = 0.0;
-    if (id >= 0 && q != 0.0) term = q * (log_q - (((double)xl - (double)m) / A.T - log_s));
-    double loss = block_sum(term, sh.red);
-    if (rest != 0.0) loss += rest * (log(rest) - (log(S.s) + gap - log_s));
-    if (empty) loss = INFINITY;
-    if (tid == 0) A.loss[r] = (float)loss;
-  }
-  if (!A.dx) return;
 
-  // ---- the gradient: p_i (Q + rest - rest / R) outside the list, p_i (Q + rest) - q_i in it
-  if (!grad || empty) {
-    const float f[VEC] = {};
-    for (int v = tid; v < R.nvec; v += blockDim.x) store_vec(R, d, same, v, f);
-    return;
-  }
-  // Relative to the other ids' own maximum, so that a share of the rest stays
-  // finite however little the student gives them.  What this writes for the
-  // listed ids is overwritten below.
-  const double wt = (double)w / A.T, all = Q + rest;
-  const float c = S.s == 0.0 ? 0.f : (float)(wt * (all * (scale / s) - rest / S.s));
-  const float mo = S.m == -INFINITY ? 0.f : S.m;
-  for (int v = tid; v < R.nvec; v += kRowThreads) {
-    float f[VEC];
-    load_vec(R, v, f);
+    // ---- the gradient: p_i (Q + rest - rest / R) outside the list, p_i (Q + rest) - q_i in it
+    const bool pass = grad && live && !empty;
+    if (A.dx && !pass) zero_slice(R, S, d, same);
+    // Relative to the other ids' own maximum, so that a share of the rest stays
+    // finite however little the student gives them.  What this writes for the
+    // listed ids is overwritten below.
+    const float mo = O.m == -INFINITY ? 0.f : O.m, zo = mo * A.a;
+    double cd = O.s == 0.0 ? 0.0 : wt * (all * (scale / s) - rest / O.s);
+    if (!isinf(zo)) cd *= exp_small(((double)zo - (double)mo * (double)A.a) * 0.693147180559945309417);
+    const float c = (float)cd;
+    auto term = [&](float x) { return c * ex2_approx(isinf(zo) ? __fsub_rn(x, mo) * A.a : fmaf(x, A.a, -zo)); };
+    auto put = [&](int v, const uint4& u) {
+      float f[VEC];
+      if (!isinf(zo)) {
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        const f32x2 a2 = f2_pack(A.a, A.a), z2 = f2_pack(-zo, -zo), c2 = f2_pack(c, c);
+        constexpr int PER = VEC / 4, WORDS = 2 / PER;  // elements a word, words a pair
 #pragma unroll
-    for (int j = 0; j < VEC; j++) f[j] = c * ex2_approx(__fsub_rn(f[j], mo) * A.a);
-    store_vec(R, d, same, v, f);
+        for (int i = 0; i < 4; i += WORDS) {
+          const float2 y = f2_unpack(f2_fma(pair_of(x[i], x[i + WORDS - 1], T()), a2, z2));
+          const float2 e = f2_unpack(f2_mul(f2_pack(ex2_approx(y.x), ex2_approx(y.y)), c2));
+          f[i * PER] = e.x;
+          f[i * PER + 1] = e.y;
+        }
+      } else {
+        unpack(u, f, T());
+#pragma unroll
+        for (int j = 0; j < VEC; j++) f[j] = term(f[j]);
+      }
+      if (same) *reinterpret_cast<uint4*>(d + (v * VEC - R.mis)) = pack(f, T());
+      else store_vec(R, d, false, v, f);
+    };
+    if (KEEP) {
+      slot = slot0;
+      for (int k = 0, v = S.w0 + tid; k < steps; k++, v += STEP) {
+        if (pass) {
+          const uint4* src = ring + slot * STEP + tid;
+          const int n = k + 1 < steps ? kBatch : last;
+#pragma unroll
+          for (int i = 0; i < kBatch; i++)
+            if (i < n) put(v + i * kRowThreads, src[i * kRowThreads]);
+        }
+        slot = slot + 1 == kDistillDepth ? 0 : slot + 1;
+        feed.next();
+      }
+    } else if (pass) {
+      const uint4* src = reinterpret_cast<const uint4*>(R.p - R.mis);
+#pragma unroll 4
+      for (int v = S.w0 + tid; v < S.w1; v += kRowThreads) put(v, src[v]);
+    }
+    if (pass) {
+      if (S.edge >= 0) d[S.edge] = from_f<T>(term(xe));
+      __syncthreads();
+      if (first) {
+        double qs = mass();
+        if (twice) {  // in the list's order, whatever the chain's
+          qs = 0.0;
+          for (int j = 0; j < K; j++)
+            if (L.id[j] == id)
+              qs += logits ? L.q[j] * exp(((double)L.m[j >> 5] - (double)top) * A.rT - log_top) : L.q[j];
+        }
+        const double p = xl == -INFINITY ? 0.0 : (double)ex2_approx(below(xl, m) * A.a) / s;
+        d[id] = from_f<T>((float)(wt * (all * p - qs)));
+      }
+    }
   }
-  __syncthreads();
-  if (first) {
-    double qs = 0.0;
-    for (int j = 0; j < K; j++)
-      if (sh.id[j] == id) qs += sh.q[j];
-    d[id] = from_f<T>((float)(wt * (all * (e / s) - qs)));
-  }
+  copies_wait<0>();
+  __syncwarp();
+  cluster_arrive();  // no CTA ends while a peer may read from it
+  cluster_wait();
 }
 
 template <typename F>
 cudaError_t by_type(int dtype, F f) {
   switch (dtype) {
-    case MS_F32: f(float()); break;
-    case MS_BF16: f(__nv_bfloat16()); break;
-    case MS_F16: f(__half()); break;
+    case MS_F32: return f(float());
+    case MS_BF16: return f(__nv_bfloat16());
+    case MS_F16: return f(__half());
     default: return cudaErrorInvalidValue;
   }
-  return cudaGetLastError();
+}
+
+cudaLaunchConfig_t row_config(int ranks, int64_t ctas, int ring, cudaStream_t stream, cudaLaunchAttribute* at) {
+  at->id = cudaLaunchAttributeClusterDimension;
+  at->val.clusterDim.x = (unsigned)ranks;
+  at->val.clusterDim.y = at->val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = (size_t)ring;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// A kernel's row clusters: how many of each size the current device runs at
+// once (0: none), asked of the driver once.  A grid of that many clusters has
+// no second wave, which would cost as much as the first.
+template <typename Args>
+cudaError_t row_clusters(void (*kernel)(Args), int ring, int ranks, int* clusters) {
+  struct Known {
+    void (*kernel)(Args);
+    int device, n[kMaxCluster + 1];
+  };
+  static std::mutex mu;
+  static std::vector<Known> known;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  for (const Known& k : known)
+    if (k.kernel == kernel && k.device == device) {
+      *clusters = k.n[ranks];
+      return cudaSuccess;
+    }
+  Known k = {kernel, device, {}};
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring);
+  // clusters beyond the portable size
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  for (int c = 1; c <= kMaxCluster && e == cudaSuccess; c++) {
+    cudaLaunchAttribute at;
+    const cudaLaunchConfig_t cfg = row_config(c, c, ring, nullptr, &at);
+    e = cudaOccupancyMaxActiveClusters(&k.n[c], kernel, &cfg);
+    if (e != cudaSuccess && c > 8) {  // a size that this device does not run
+      cudaGetLastError();
+      k.n[c] = 0;
+      e = cudaSuccess;
+    }
+  }
+  if (e != cudaSuccess) return e;
+  known.push_back(k);
+  *clusters = k.n[ranks];
+  return cudaSuccess;
+}
+
+// Launches a row kernel with the best CTAs a row, `fit` or more.  The rows go
+// over the clusters in rounds, so the time is about rounds * (slice + what a
+// row costs its CTAs beside the copies), in bytes at a CTA's share of the
+// bandwidth.
+template <typename Args>
+cudaError_t launch_rows(void (*kernel)(Args), const Args& A, int64_t row_bytes, int fit, int ring,
+                        cudaStream_t stream) {
+  int best = 0, best_clusters = 0;
+  int64_t least = INT64_MAX;
+  for (int c = fit; c <= kMaxCluster; c++) {
+    int n = 0;
+    const cudaError_t e = row_clusters(kernel, ring, c, &n);
+    if (e != cudaSuccess) return e;
+    if (n < 1) continue;
+    const int64_t cost = (A.B + n - 1) / n * (row_bytes / c + (c == 1 ? 16384 : 24576 + 2048 * c));
+    if (cost < least) {
+      least = cost;
+      best = c;
+      best_clusters = n;
+    }
+  }
+  if (best == 0) return cudaErrorInvalidConfiguration;
+  cudaLaunchAttribute at;
+  const cudaLaunchConfig_t cfg = row_config(best, std::min<int64_t>(A.B, best_clusters) * best, ring, stream, &at);
+  return cudaLaunchKernelEx(&cfg, kernel, A);
 }
 
 }  // namespace
 
 cudaError_t launch_logprobs(const ScoreArgs& A, int dtype, cudaStream_t stream) {
-  return by_type(dtype, [&](auto t) { logprobs_kernel<decltype(t)><<<(unsigned)A.B, kRowThreads, 0, stream>>>(A); });
+  return by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const bool ent = A.out.entropy != nullptr, top = A.top_n > 0;
+    auto k = ent ? (top ? logprobs_kernel<T, true, true> : logprobs_kernel<T, true, false>)
+                 : (top ? logprobs_kernel<T, false, true> : logprobs_kernel<T, false, false>);
+    // the bounds want twice as many threads a row as alternatives
+    const int fit = A.top_n > kRowThreads / 2 ? 2 : 1;
+    return launch_rows(k, A, (int64_t)A.V * sizeof(T), fit, kScoreRing, stream);
+  });
 }
 
 // CTAs a row of the backward grid: one vector more than V / VEC, as a row may
@@ -609,11 +1422,22 @@ cudaError_t launch_logprobs_backward(const ScoreArgs& A, int dtype, cudaStream_t
     using T = decltype(t);
     const int chunks = (int)grad_chunks(A.V, Row<T>::VEC);
     logprobs_backward_kernel<T><<<(unsigned)(A.B * chunks), kGradThreads, 0, stream>>>(A, chunks);
+    return cudaGetLastError();
   });
 }
 
 cudaError_t launch_distill(const DistillArgs& A, int dtype, cudaStream_t stream) {
-  return by_type(dtype, [&](auto t) { distill_kernel<decltype(t)><<<(unsigned)A.B, kRowThreads, 0, stream>>>(A); });
+  return by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    // a vector more than V / VEC, as a row may start anywhere in its first
+    const int64_t vecs = ((int64_t)A.V + 2 * Row<T>::VEC - 2) / Row<T>::VEC, held = kDistillRing / 16;
+    int fit = 1;
+    while (fit < kMaxCluster && (vecs + fit - 1) / fit > held) fit++;
+    const bool keep = A.dx && (vecs + fit - 1) / fit <= held;
+    if (!A.dx) fit = 1;
+    return launch_rows(keep ? distill_kernel<T, true> : distill_kernel<T, false>, A, (int64_t)A.V * sizeof(T), fit,
+                       kDistillRing, stream);
+  });
 }
 
 }  // namespace ms

@@ -174,7 +174,7 @@ def distill(x, T, ids, values, kind, weight, dtype):
         log_R, tail = -np.inf, 0.0
     if rest > 0:
         loss += rest * (math.log(rest) - log_R)
-    eps_s = eps_t * tail  # the listed ids' terms are in fp64
+    eps_s = R.eps_s  # the listed ids' terms are fp32 terms like the others
     b_loss = 0.0
     if np.isfinite(loss):
         b_loss = (Q + rest) * eps_s + rest * eps_t + abs(loss) * U + 1e-12
@@ -182,7 +182,8 @@ def distill(x, T, ids, values, kind, weight, dtype):
         return loss, b_loss, zero, zero
     all_ = Q + rest
     dx = np.where(listed, R.p * all_ - mass, 0.0)
-    b = np.where(listed, R.p * all_ * eps_s + 1e-13, 0.0)
+    far = np.where(R.p > 0, -R.d, 0.0)
+    b = np.where(listed, R.p * all_ * (eps_s + (3 * far + 4) * U) + 1e-13, 0.0)
     if not tail_empty:
         share = np.zeros(V)
         share[~listed] = po
