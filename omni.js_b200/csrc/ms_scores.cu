@@ -43,7 +43,8 @@ constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kBatch = 4;       // 16-byte vectors of a thread's step
 constexpr int kMaxCluster = 16;
-constexpr int kBuf = 1024;      // keys the selection holds: top_n (<= 256) and at least one tile of kRowThreads
+constexpr int kBuf = 992;       // keys the selection holds (runs of 32)
+constexpr int kScan = 512;      // of them, those that the tiled selection uses: top_n and a tile of kRowThreads
 
 // ---------------------------------------------------------------- row access
 // A row is read in 16-byte vectors on 16-byte boundaries, whatever its start:
@@ -157,6 +158,7 @@ typedef unsigned long long f32x2;
 struct Sums {
   float m = -INFINITY, z = 0.f;
   f32x2 s = 0, q = 0;
+  bool odd = false;  // masked elements (0 times their y of -Inf), or m a beyond fp32: each term with care from here on
 };
 
 // y, bounded below so that a term of 0 times it is 0 (a NaN stays one)
@@ -234,38 +236,38 @@ __device__ __forceinline__ void add_words(Sums& t, const uint32_t (&w)[N], float
   constexpr int PER = sizeof(T) == 4 ? 2 : 1;  // words a pair
   const float hi = largest(w, T());
   if (hi > t.m) raise_to<ENT>(t, hi, a);
-  const f32x2 z2 = f2_pack(-t.z, -t.z), a2 = f2_pack(a, a);
-  f32x2 s = t.s, q = t.q;
-#pragma unroll
-  for (int i = 0; i < N; i += PER) {
-    const f32x2 y2 = f2_fma(pair_of(w[i], w[i + PER - 1], T()), a2, z2);
-    const float2 y = f2_unpack(y2);
-    const f32x2 e = f2_pack(ex2_approx(y.x), ex2_approx(y.y));
-    s = f2_add(s, e);
-    if constexpr (ENT) q = f2_fma(e, y2, q);
-  }
-  // 0 times the y of a masked element, or an m a beyond fp32: once more, with care
-  bool odd = isinf(t.z);
-  if constexpr (ENT) {
-    const float2 h = f2_unpack(q);
-    odd |= isnan(h.x + h.y);
-  }
-  if (odd) {
-    const float m = t.m == -INFINITY ? 0.f : t.m;
-    s = t.s;
-    q = t.q;
+  if (!t.odd) {
+    const f32x2 z2 = f2_pack(-t.z, -t.z), a2 = f2_pack(a, a);
+    f32x2 s = t.s, q = t.q;
 #pragma unroll
     for (int i = 0; i < N; i += PER) {
-      const float2 x = f2_unpack(pair_of(w[i], w[i + PER - 1], T()));
-      const float y0 = bounded(isinf(t.z) ? __fsub_rn(x.x, m) * a : fmaf(x.x, a, -t.z));
-      const float y1 = bounded(isinf(t.z) ? __fsub_rn(x.y, m) * a : fmaf(x.y, a, -t.z));
-      const f32x2 e = f2_pack(ex2_approx(y0), ex2_approx(y1));
+      const f32x2 y2 = f2_fma(pair_of(w[i], w[i + PER - 1], T()), a2, z2);
+      const float2 y = f2_unpack(y2);
+      const f32x2 e = f2_pack(ex2_approx(y.x), ex2_approx(y.y));
       s = f2_add(s, e);
-      if constexpr (ENT) q = f2_fma(e, f2_pack(y0, y1), q);
+      if constexpr (ENT) q = f2_fma(e, y2, q);
+    }
+    t.odd = isinf(t.z);
+    if constexpr (ENT) {
+      const float2 h = f2_unpack(q);
+      t.odd |= isnan(h.x + h.y);
+    }
+    if (!t.odd) {
+      t.s = s;
+      t.q = q;
+      return;
     }
   }
-  t.s = s;
-  t.q = q;
+  const float m = t.m == -INFINITY ? 0.f : t.m;
+#pragma unroll
+  for (int i = 0; i < N; i += PER) {
+    const float2 x = f2_unpack(pair_of(w[i], w[i + PER - 1], T()));
+    const float y0 = bounded(isinf(t.z) ? __fsub_rn(x.x, m) * a : fmaf(x.x, a, -t.z));
+    const float y1 = bounded(isinf(t.z) ? __fsub_rn(x.y, m) * a : fmaf(x.y, a, -t.z));
+    const f32x2 e = f2_pack(ex2_approx(y0), ex2_approx(y1));
+    t.s = f2_add(t.s, e);
+    if constexpr (ENT) t.q = f2_fma(e, f2_pack(y0, y1), t.q);
+  }
 }
 
 template <bool ENT>
@@ -316,7 +318,7 @@ __device__ __forceinline__ RowSums exact_sums(float4 w, float a) {
   return r;
 }
 
-// The sums of lanes 0 to 15's parts (m = -Inf, s = q = 0 for none) in every lane.
+// The sums of the lanes' parts (m = -Inf, s = q = 0 for none) in every lane.
 template <bool ENT>
 __device__ __forceinline__ RowSums lane_sums(const RowSums& p, float a) {
   RowSums r;
@@ -326,20 +328,28 @@ __device__ __forceinline__ RowSums lane_sums(const RowSums& p, float a) {
   r.q = (p.q + p.s * (double)d * 0.693147180559945309417) * c;
   r.s = p.s * c;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
+  for (int o = 16; o > 0; o >>= 1) {
     r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
     if constexpr (ENT) r.q += __shfl_xor_sync(0xffffffffu, r.q, o);
   }
-  r.s = __shfl_sync(0xffffffffu, r.s, 0);
-  if constexpr (ENT) r.q = __shfl_sync(0xffffffffu, r.q, 0);
   return r;
 }
 
-// The sums of the CTA's warps, from w[kRowWarps] in shared memory.
-template <bool ENT>
-__device__ __forceinline__ RowSums join_warps(const float4* w, float a) {
+// The sums of n warps, warp(i) being the i-th's.
+template <bool ENT, typename Warp>
+__device__ __forceinline__ RowSums join_warps(int n, float a, Warp warp) {
   const int lane = threadIdx.x & 31;
-  return lane_sums<ENT>(lane < kRowWarps ? exact_sums(w[lane], a) : RowSums{-INFINITY, 0.0, 0.0}, a);
+  RowSums r = {-INFINITY, 0.0, 0.0};
+  if (lane < n) r = exact_sums(warp(lane), a);
+  r = lane_sums<ENT>(r, a);
+#pragma unroll 1
+  for (int i = 32; i < n; i += 32) {
+    RowSums p = {-INFINITY, 0.0, 0.0};
+    if (i + lane < n) p = exact_sums(warp(i + lane), a);
+    p = lane_sums<ENT>(p, a);
+    r = lane_sums<ENT>(lane == 0 ? r : lane == 1 ? p : RowSums{-INFINITY, 0.0, 0.0}, a);
+  }
+  return r;
 }
 
 // Named barriers: the warps that only tell others something do not wait.
@@ -368,9 +378,11 @@ struct Slice {
     if (edge >= R.V) edge = -1;
   }
   __device__ __forceinline__ int steps() const { return (w1 - w0 + kBatch * kRowThreads - 1) / (kBatch * kRowThreads); }
-  // vectors that this thread has in the last step (kBatch or fewer; less than 1 for none)
-  __device__ __forceinline__ int last() const {
-    return (w1 - w0 - (steps() - 1) * kBatch * kRowThreads - (int)threadIdx.x + kRowThreads - 1) / kRowThreads;
+  // how many of them the thread has in full, and its vectors in the one after those (none: 0)
+  __device__ __forceinline__ int whole_steps(int* rest) const {
+    const int n = max(0, (w1 - w0 - (int)threadIdx.x + kRowThreads - 1) / kRowThreads);  // its vectors
+    *rest = n % kBatch;
+    return n / kBatch;
   }
   // the thread that holds element i, or -1 when it is not the slice's
   __device__ __forceinline__ int owner(const Row<T>& R, int i, int rank, int ranks) const {
@@ -392,16 +404,6 @@ template <int N>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-template <int MOST>
-__device__ __forceinline__ void copies_wait(int n) {
-  if constexpr (MOST > 0) {
-    if (n >= MOST) copies_wait<MOST>();
-    else copies_wait<MOST - 1>(n);
-  } else {
-    copies_wait<0>();
-  }
-}
-
 // The rows first, first + step, ... that a cluster works on, and which of them
 // are read at all: those with an id inside [0, V) in their list of n (every row
 // when n = 0), and, where `weight` is given, a weight other than 0.  The row
@@ -432,24 +434,42 @@ struct RowList {
   }
 };
 
+// The ring's places go round: the step that was just worked on frees the place
+// that the feed fills next.
+template <int DEPTH>
+struct Place {
+  uint32_t at, begin;  // the thread's first vector of the step, in shared memory
+  __device__ __forceinline__ explicit Place(uint32_t first) : at(first), begin(first) {}
+  __device__ __forceinline__ void next() {
+    at += kBatch * kRowThreads * 16;
+    if (at == begin + DEPTH * kBatch * kRowThreads * 16) at = begin;
+  }
+};
+
 // The copies of a thread's vectors, in the order of the rows and of their
-// steps, one group a step (an empty one when the rows are through).
-template <typename T, int DEPTH>
+// steps, one group a step (an empty one when the rows are through).  TWICE:
+// each row a second time, from its last step to its first, so that what was
+// read last, which L2 still holds, comes first.
+template <typename T, int DEPTH, bool TWICE = false>
 struct Feed {
   RowList rows;
   const void* x;
   int64_t ld, row;
-  int rank, ranks, left, last, slot;
+  int rank, ranks;
+  int run, left;           // the pass's whole steps to come, and steps (0 or 1) after the whole ones
+  int whole, part, rest;   // the row's whole steps, steps after them and vectors in that
+  bool again;         // in the row's second pass
   const uint4* src;   // the thread's next vector
-  uint32_t ring;      // the thread's first place in shared memory
-  __device__ __forceinline__ void start(int64_t first) {
+  // from the row that rows has fetched
+  __device__ __forceinline__ void start(int64_t first, Place<DEPTH> place) {
     row = first;
-    slot = 0;
-    left = 0;
-    rows.fetch(row);
+    run = left = 0;
     settle();
 #pragma unroll 1
-    for (int i = 0; i < DEPTH; i++) next();
+    for (int i = 0; i < DEPTH; i++) {
+      next(place.at);
+      place.next();
+    }
   }
   // the next row, from `row` on, that is read and has vectors here
   __device__ __forceinline__ void settle() {
@@ -460,44 +480,65 @@ struct Feed {
         const Row<T> R(x, row, ld, rows.V);
         const Slice<T> S(R, rank, ranks);
         src = reinterpret_cast<const uint4*>(R.p - R.mis) + S.w0 + threadIdx.x;
-        left = S.steps();
-        last = S.last();
-        if (left > 0) return;
+        run = whole = S.whole_steps(&rest);
+        left = part = S.steps() - whole;
+        again = false;
+        if (run + left > 0) return;
       }
       row += rows.step;
     }
   }
-  __device__ __forceinline__ void next() {
-    if (left > 0) {
-      const uint32_t dst = ring + slot * (kBatch * kRowThreads * 16);
-      if (left > 1) {
+  __device__ __forceinline__ void next(uint32_t dst) {
+    bool end = false;  // of the pass: at the same call in every thread, however its last steps are made up
+    if (run > 0) {
 #pragma unroll
-        for (int i = 0; i < kBatch; i++) copy16(dst + i * (kRowThreads * 16), src + i * kRowThreads);
-        src += kBatch * kRowThreads;
-        left--;
-      } else {
+      for (int i = 0; i < kBatch; i++) copy16(dst + i * (kRowThreads * 16), src + i * kRowThreads);
+      src += TWICE && again ? -kBatch * kRowThreads : kBatch * kRowThreads;
+      end = --run == 0 && left == 0;
+    } else if (left > 0) {  // the step that the thread has in part, or not at all
 #pragma unroll
-        for (int i = 0; i < kBatch; i++)
-          if (i < last) copy16(dst + i * (kRowThreads * 16), src + i * kRowThreads);
-        left = 0;
-        row += rows.step;
-        settle();
+      for (int i = 0; i + 1 < kBatch; i++)
+        if (i < rest) copy16(dst + i * (kRowThreads * 16), src + i * kRowThreads);
+      left = 0;
+      end = true;
+      if (TWICE && again && whole > 0) {
+        run = whole;
+        src -= kBatch * kRowThreads;
+        end = false;
       }
     }
-    slot = slot + 1 == DEPTH ? 0 : slot + 1;
     copies_end_group();
+    if (end) turn();
+  }
+  // the end of a pass
+  __device__ __forceinline__ void turn() {
+    if (TWICE && !again) {
+      again = true;
+      // the second pass begins with the step that comes after the whole ones,
+      // where src is; without one, with the last of those
+      left = part;
+      if (left == 0) {
+        run = whole;
+        src -= kBatch * kRowThreads;
+      }
+      return;
+    }
+    row += rows.step;
+    settle();
   }
 };
 
-// The words of a step's vectors out of the ring, those beyond the first n
-// vectors being elements of -Inf.
-template <typename T>
-__device__ __forceinline__ void ring_step(const uint4* src, int n, uint32_t (&w)[4 * kBatch]) {
-  constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
+// One vector out of the ring.
+__device__ __forceinline__ uint4 ring_vec(uint32_t at) {
+  uint4 u;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
+  return u;
+}
+// A whole step's words.
+__device__ __forceinline__ void ring_step(uint32_t at, uint32_t (&w)[4 * kBatch]) {
 #pragma unroll
   for (int i = 0; i < kBatch; i++) {
-    uint4 u = make_uint4(none, none, none, none);
-    if (i < n) u = src[i * kRowThreads];
+    const uint4 u = ring_vec(at + i * (kRowThreads * 16));
     w[4 * i] = u.x;
     w[4 * i + 1] = u.y;
     w[4 * i + 2] = u.z;
@@ -507,11 +548,11 @@ __device__ __forceinline__ void ring_step(const uint4* src, int n, uint32_t (&w)
 
 // Element l of a thread's step (its vectors lie kRowThreads vectors apart, l
 // counting elements of memory from the first one) set to -Inf.
-template <typename T>
-__device__ __forceinline__ void mask_element(uint32_t (&w)[4 * kBatch], int l) {
+template <typename T, int N>
+__device__ __forceinline__ void mask_element(uint32_t (&w)[N], int l) {
   constexpr int VEC = Row<T>::VEC, PER = VEC / 4;
 #pragma unroll
-  for (int i = 0; i < 4 * kBatch; i++) {
+  for (int i = 0; i < N; i++) {
     const int at = (i / 4) * (kRowThreads * VEC) + (i % 4) * PER;  // the word's first element
     if constexpr (PER == 1) {
       if (l == at) w[i] = 0xff800000u;
@@ -547,13 +588,12 @@ __device__ __forceinline__ void sort_desc(unsigned long long* k, int n) {
   __syncthreads();
 }
 
-constexpr int kRank = 512;  // keys up to which counting the larger ones is faster than sorting
-
 struct TopSmem {
   unsigned long long key[kBuf];
   int n;
 };
 
+constexpr int kAlone = 10;
 constexpr int kRounds = kScoreMax / kRowWarps;  // bounds that a CTA gives for the largest top_n
 
 // A warp's share of the bounds for the alternatives: its j-th largest thread
@@ -586,31 +626,93 @@ __device__ __forceinline__ float row_bound(const float* lists, int ranks, int to
   return best <= fkey(-INFINITY) ? -INFINITY : fkey_inv(best);
 }
 
+// A warp's keys, one a lane, sorted largest first.
+__device__ __forceinline__ unsigned long long warp_sort_desc(unsigned long long k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int st = size >> 1; st > 0; st >>= 1) {
+      const unsigned long long o = __shfl_xor_sync(0xffffffffu, k, st);
+      const bool first = (lane & st) == 0, down = (lane & size) == 0;
+      k = (first == down) == (k > o) ? k : o;
+    }
+  }
+  return k;
+}
+
+// n keys (n <= kBuf) in runs of 32, each sorted by a warp.
+__device__ __forceinline__ void sort_runs(TopSmem& sh, int n) {
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i - lane < n; i += kRowThreads)
+    sh.key[i] = warp_sort_desc(i < n ? sh.key[i] : 0ull);
+  __syncthreads();
+}
+
+// put(place, key) for each of the first top_n of n keys in sorted runs: a key's
+// place is its place in its run and the number of larger keys in each of the
+// others.  The places beyond the keys get 0.
+template <typename Put>
+__device__ __forceinline__ void place_keys(const TopSmem& sh, int n, int top_n, Put put) {
+  const int runs = (n + 31) / 32;
+  for (int i = threadIdx.x; i < n; i += kRowThreads) {
+    const unsigned long long k = sh.key[i];
+    int place = i & 31;
+#pragma unroll 4
+    for (int q = 0; q < runs; q++) {
+      const unsigned long long* run = sh.key + q * 32;
+      int at = 0;
+#pragma unroll
+      for (int st = 16; st > 0; st >>= 1) at += run[at + st - 1] > k ? st : 0;
+      at += run[at] > k;
+      if (q != i / 32) place += at;
+    }
+    if (place < top_n) put(place, k);
+  }
+  for (int i = n + threadIdx.x; i < top_n; i += kRowThreads) put(i, 0ull);
+}
+
+// Who holds a CTA's elements that reach the bound.
+struct TopOwners {
+  uint8_t thread[kRowThreads];
+};
+
 // The CTA's elements >= bound, as keys into the buffer `to` (a peer's): only
-// threads whose maximum reaches the bound hold any, and the warp reads each
-// such thread's vectors again together.  Keys beyond the buffer are counted
-// and left out.  xe: the thread's edge element.
+// threads whose maximum reaches the bound hold any, and all threads read those
+// threads' vectors again together, several in flight each.  Keys beyond the
+// buffer are counted and left out.  xe: the thread's edge element.
 template <typename T>
 __device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, float tm, float xe, float bound,
-                                           TopSmem* to) {
-  constexpr int VEC = Row<T>::VEC;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+                                           TopOwners& own, int& owners, TopSmem* to) {
+  constexpr int VEC = Row<T>::VEC, AHEAD = 4;
   auto take = [&](float x, int i) {
     if (x >= bound && x > -INFINITY) {
       const int n = atomicAdd(&to->n, 1);
       if (n < kBuf) to->key[n] = top_key(x, i);
     }
   };
+  if (tm >= bound && tm > -INFINITY) own.thread[atomicAdd(&owners, 1)] = (uint8_t)threadIdx.x;
   if (S.edge >= 0) take(xe, S.edge);
-  unsigned who = __ballot_sync(0xffffffffu, tm >= bound && tm > -INFINITY);
-  while (who) {
-    const int owner = warp * 32 + __ffs(who) - 1;
-    who &= who - 1;
-    for (int v = S.w0 + owner + lane * kRowThreads; v < S.w1; v += 32 * kRowThreads) {
-      float f[VEC];
-      load_vec(R, v, f);
+  __syncthreads();
+  const int n = owners, each = (S.w1 - S.w0 + kRowThreads - 1) / kRowThreads;
+  const uint4* base = reinterpret_cast<const uint4*>(R.p - R.mis);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n * each; i += AHEAD * kRowThreads) {
+    uint4 u[AHEAD];
+    int v[AHEAD];
 #pragma unroll
-      for (int j = 0; j < VEC; j++) take(f[j], v * VEC - R.mis + j);
+    for (int a = 0; a < AHEAD; a++) {
+      const int it = i + a * kRowThreads, k = it / n;
+      v[a] = it < n * each ? S.w0 + own.thread[it - k * n] + k * kRowThreads : INT_MAX;
+      if (v[a] < S.w1) u[a] = base[v[a]];
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; a++) {
+      if (v[a] >= S.w1) continue;
+      float f[VEC];
+      unpack(u[a], f, T());
+#pragma unroll
+      for (int j = 0; j < VEC; j++) take(f[j], v[a] * VEC - R.mis + j);
     }
   }
 }
@@ -642,9 +744,9 @@ __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
       __syncthreads();
       const int n = sh.n;
       __syncthreads();
-      if (n + (int)blockDim.x > kBuf) {
-        for (int i = n + threadIdx.x; i < kBuf; i += blockDim.x) sh.key[i] = 0;
-        sort_desc(sh.key, kBuf);
+      if (n + (int)blockDim.x > kScan) {
+        for (int i = n + threadIdx.x; i < kScan; i += blockDim.x) sh.key[i] = 0;
+        sort_desc(sh.key, kScan);
         thr = sh.key[top_n - 1];
         __syncthreads();
         if (threadIdx.x == 0) sh.n = top_n;
@@ -653,8 +755,8 @@ __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
     }
   }
   const int n = sh.n;
-  for (int i = n + threadIdx.x; i < kBuf; i += blockDim.x) sh.key[i] = 0;
-  sort_desc(sh.key, kBuf);
+  for (int i = n + threadIdx.x; i < kScan; i += blockDim.x) sh.key[i] = 0;
+  sort_desc(sh.key, kScan);
 }
 
 // ---------------------------------------------------------------- forward
@@ -668,13 +770,18 @@ struct ScoreJoin {
   float4 warp[2][kRowWarps];
   RowSums cta[2][kMaxCluster];
 };
+// With alternatives: every warp's sums go to rank 0 as they are.
 struct TopJoin {
-  float bound[2][kRounds];              // what the CTA tells the others
+  float red[kRounds][kRowWarps];   // then in red[.][0] the bounds that the CTA tells the others
   union {
-    float red[kRounds][kRowWarps];      // before the CTAs meet
-    float lists[kRowThreads];           // what they all told, after it
+    float lists[4 * kRounds];      // what they all told
+    TopOwners own;
   };
-  TopSmem sel;                          // rank 0's is the row's
+  int owners;
+  float m;                         // the row's maximum and log of its sum
+  double s, log_s;
+  float warps[kMaxCluster * kRowWarps][3];  // every warp's {m, s, q}
+  TopSmem sel;                     // rank 0's is the row's
 };
 
 // A padded row's outputs, by one warp.
@@ -702,18 +809,23 @@ __device__ __forceinline__ double log_sum(double s) {
 
 // A row's numbers and its tokens' log-probabilities from its sums, by one warp.
 // log s is -Inf for a row of -Inf alone, NaN for a NaN row.
+// y, x: lane t's token and its logit, t < 32.
 template <typename T, bool ENT>
-__device__ __forceinline__ void write_row(const ScoreArgs& A, int64_t r, const Row<T>& R, const RowSums& sum) {
+__device__ __forceinline__ void write_row(const ScoreArgs& A, int64_t r, const Row<T>& R, const RowSums& sum, int y,
+                                          float x) {
   const ms_scores& O = A.out;
   const int lane = threadIdx.x & 31;
   const double log_s = sum.s == 0.0 ? -INFINITY : log_sum(sum.s);
   const bool empty = sum.s == 0.0;
   if (O.logprobs)
     for (int t = lane; t < A.n_tok; t += 32) {
-      const int y = A.tokens[r * A.n_tok + t];
+      if (t >= 32) {
+        y = A.tokens[r * A.n_tok + t];
+        x = (uint32_t)y < (uint32_t)A.V ? to_f(R.p[y]) : 0.f;
+      }
       float lp = 0.f;
       if ((uint32_t)y < (uint32_t)A.V)
-        lp = empty ? -INFINITY : (float)(((double)to_f(R.p[y]) - (double)sum.m) * A.rT - log_s);
+        lp = empty ? -INFINITY : (float)(((double)x - (double)sum.m) * A.rT - log_s);
       O.logprobs[r * A.n_tok + t] = lp;
     }
   if (lane == 0) {
@@ -739,31 +851,34 @@ __device__ __forceinline__ void write_row(const ScoreArgs& A, int64_t r, const R
 template <typename T, bool ENT, bool TOP>
 __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(ScoreArgs A) {
   extern __shared__ uint4 ring[];
-  __shared__ ScoreJoin join;
-  __shared__ std::conditional_t<TOP, TopJoin, int> top_smem;
-  TopJoin& tp = reinterpret_cast<TopJoin&>(top_smem);
+  __shared__ std::conditional_t<TOP, TopJoin, ScoreJoin> joins;
+  TopJoin& tp = reinterpret_cast<TopJoin&>(joins);
+  ScoreJoin& join = reinterpret_cast<ScoreJoin&>(joins);
   TopSmem* const top = &tp.sel;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), ranks = (int)cl.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // bounds that the alternatives need, and those that each CTA tells: twice its share and two more
   const int rounds = (A.top_n + kRowWarps - 1) / kRowWarps;
-  const int told = ranks == 1 ? rounds : min(rounds, (2 * rounds + ranks - 1) / ranks + 2);
+  const int share = min(rounds, (2 * rounds + ranks - 1) / ranks + 2);
+  // with few CTAs or alternatives each CTA's own bound leaves few enough elements
+  const bool alone = ranks * rounds <= kAlone;
+  const int told = alone ? rounds : share;
   const int64_t first = blockIdx.x / ranks, step = gridDim.x / ranks;
   const ms_scores& O = A.out;
   Feed<T, kScoreDepth> feed;
   feed.rows = {A.tokens, nullptr, A.n_tok, A.V, A.B, step, -1, 1.f};
+  feed.rows.fetch(first);
   RowList rows = feed.rows;  // the rows as they are worked on
   feed.x = A.x;
   feed.ld = A.ld;
   feed.rank = rank;
   feed.ranks = ranks;
-  feed.ring = smem_addr(ring + tid);
-  feed.start(first);
-  rows.fetch(first);
-  int slot = 0, which = 0, turn_rank = 0, turn_warp = 0;
-  cluster_arrive();
-  bool waiting = true;  // for the cluster's barrier of the row before (at first: for its CTAs to have started)
+  Place<kScoreDepth> place(smem_addr(ring + tid));
+  feed.start(first, place);
+  int which = 0, turn_rank = 0, turn_warp = 0;
+  if constexpr (!TOP) cluster_arrive();
+  bool waiting = !TOP;  // for the cluster's barrier of the row before (at first: for its CTAs to have started)
   for (int64_t r = first; r < A.B; r += step) {
     const bool live = rows.read(r);  // the same in every CTA of the cluster
     rows.fetch(r + step);
@@ -774,29 +889,49 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
     const Row<T> R(A.x, r, A.ld, A.V);
     const Slice<T> S(R, rank, ranks);
     const float xe = S.edge >= 0 ? to_f(R.p[S.edge]) : -INFINITY;
-    if (TOP && tid == 0) top->n = 0;
+    if constexpr (TOP) {
+      if (tid == 0) top->n = tp.owners = 0;
+      cluster_arrive();
+    }
+    // the warp that writes the row's numbers
+    const bool writes = TOP ? rank == 0 && warp == kRowWarps - 1 : rank == turn_rank && warp == turn_warp;
+    int y = -1;
+    if (writes && lane < A.n_tok) y = A.tokens[r * A.n_tok + lane];
+    const float xy = (uint32_t)y < (uint32_t)A.V ? to_f(R.p[y]) : 0.f;
 
     Sums t;
-    const int steps = S.steps(), last = S.last();
-    for (int k = 1; k <= steps; k++) {
+    int rest;
+    const int whole = S.whole_steps(&rest);
+#pragma unroll 1
+    for (int k = 0; k < whole; k++) {
       copies_wait<kScoreDepth - 1>();
       uint32_t w[4 * kBatch];
-      ring_step<T>(ring + slot * (kBatch * kRowThreads) + tid, k < steps ? kBatch : last, w);
-      slot = slot + 1 == kScoreDepth ? 0 : slot + 1;
+      ring_step(place.at, w);
       add_words<T, 4 * kBatch, ENT>(t, w, A.a);
-      feed.next();
+      feed.next(place.at);
+      place.next();
+    }
+    if (whole < S.steps()) {
+      copies_wait<kScoreDepth - 1>();
+#pragma unroll 1
+      for (int i = 0; i < rest; i++) {
+        const uint4 u = ring_vec(place.at + i * (kRowThreads * 16));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        add_words<T, 4, ENT>(t, w, A.a);
+      }
+      feed.next(place.at);
+      place.next();
     }
     if (S.edge >= 0) add_term<ENT>(t, xe, A.a);
     const float4 ws = warp_sums<ENT>(t, A.a);
-    if (lane == 0) join.warp[which][warp] = ws;
-
     if constexpr (!TOP) {
+      if (lane == 0) join.warp[which][warp] = ws;
       __syncwarp();
       if (warp == turn_warp) {
         bar_sync(1 + which);
-        const RowSums mine = join_warps<ENT>(join.warp[which], A.a);
+        const RowSums mine = join_warps<ENT>(kRowWarps, A.a, [&](int i) { return join.warp[which][i]; });
         if (waiting) cluster_wait();
-        if (ranks == 1) write_row<T, ENT>(A, r, R, mine);
+        if (ranks == 1) write_row<T, ENT>(A, r, R, mine, y, xy);
         else if (lane == 0) *cl.map_shared_rank(&join.cta[which][rank], turn_rank) = mine;
         __syncwarp();
       } else {
@@ -805,11 +940,11 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
       }
       cluster_arrive();
       waiting = true;
-      if (ranks > 1 && rank == turn_rank && warp == turn_warp) {
+      if (ranks > 1 && writes) {
         cluster_wait();
         waiting = false;
         const RowSums sum = lane_sums<ENT>(lane < ranks ? join.cta[which][lane] : RowSums{-INFINITY, 0.0, 0.0}, A.a);
-        write_row<T, ENT>(A, r, R, sum);
+        write_row<T, ENT>(A, r, R, sum, y, xy);
       }
       which ^= 1;
       if (++turn_rank == ranks) {
@@ -819,66 +954,68 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
     } else {
       top_maxima(t.m, told, tp.red);
       __syncthreads();
-      if (waiting) cluster_wait();
-      waiting = false;
-      if (warp == 0) {
-        const RowSums mine = join_warps<ENT>(join.warp[which], A.a);
-        if (lane < told) {
-          float b = tp.red[lane][0];
+      cluster_wait();  // rank 0 is at this row
+      float bound;
+      if (alone) {
+        bound = tp.red[rounds - 1][0];
 #pragma unroll
-          for (int w = 1; w < kRowWarps; w++) b = fminf(b, tp.red[lane][w]);
-          tp.bound[which][lane] = b;
+        for (int w = 1; w < kRowWarps; w++) bound = fminf(bound, tp.red[rounds - 1][w]);
+      } else {
+        if (tid < told) {
+          float b = tp.red[tid][0];
+#pragma unroll
+          for (int w = 1; w < kRowWarps; w++) b = fminf(b, tp.red[tid][w]);
+          tp.red[tid][0] = b;
         }
-        if (lane == 0) *cl.map_shared_rank(&join.cta[which][rank], 0) = mine;
         __syncwarp();
-      }
-      cluster_arrive();
-      cluster_wait();
-      float bound = tp.bound[which][rounds - 1];
-      if (ranks > 1) {
-        if (tid < ranks * told) tp.lists[tid] = cl.map_shared_rank(tp.bound[which], tid / told)[tid % told];
+        cluster_arrive();
+        cluster_wait();
+        if (tid < ranks * told) tp.lists[tid] = cl.map_shared_rank(&tp, tid / told)->red[tid % told][0];
         __syncthreads();
         bound = row_bound(tp.lists, ranks, told, rounds);
+        __syncthreads();  // the lists' place is the owners' next
       }
-      top_gather(R, S, t.m, xe, bound, cl.map_shared_rank(top, 0));
+      if (lane < 3) cl.map_shared_rank(&tp, 0)->warps[rank * kRowWarps + warp][lane] = lane == 0 ? ws.x : lane == 1 ? ws.z : ws.w;
+      top_gather(R, S, t.m, xe, bound, tp.own, tp.owners, cl.map_shared_rank(top, 0));
       __syncwarp();
       cluster_arrive();
       cluster_wait();  // the gathered keys are rank 0's
-      const int now = which;
-      which ^= 1;
       if (rank != 0) continue;
-      const RowSums sum = lane_sums<ENT>(lane < ranks ? join.cta[now][lane] : RowSums{-INFINITY, 0.0, 0.0}, A.a);
-      if (warp == kRowWarps - 1) write_row<T, ENT>(A, r, R, sum);
-      const double log_s = log_sum(sum.s);
-      auto logprob = [&](float x) { return (float)(((double)x - (double)sum.m) * A.rT - log_s); };
-      const bool bad = !(sum.s >= 0.0);
+      if (writes) {
+        const RowSums sum = join_warps<ENT>(ranks * kRowWarps, A.a, [&](int i) {
+          const float m = tp.warps[i][0];
+          return make_float4(m, m == -INFINITY ? 0.f : m * A.a, tp.warps[i][1], tp.warps[i][2]);
+        });
+        if (lane == 0) {
+          tp.m = sum.m;
+          tp.s = sum.s;
+          tp.log_s = log_sum(sum.s);
+        }
+        write_row<T, ENT>(A, r, R, sum, y, xy);
+      }
       const int n = top->n;
+      bool bad = false;  // known once the warp above is done
       auto put = [&](int i, unsigned long long k) {
         if (O.top_ids) O.top_ids[r * A.top_n + i] = k ? (int32_t)~(uint32_t)k : -1;
-        if (O.top_logprobs)
-          O.top_logprobs[r * A.top_n + i] = k ? logprob(fkey_inv((uint32_t)(k >> 32))) : (bad ? (float)sum.s : -INFINITY);
+        if (O.top_logprobs) {
+          const double x = (double)fkey_inv((uint32_t)(k >> 32));
+          O.top_logprobs[r * A.top_n + i] =
+              k ? (float)((x - (double)tp.m) * A.rT - tp.log_s) : (bad ? (float)tp.s : -INFINITY);
+        }
       };
+      if (n > kBuf) {  // rows whose largest elements crowd into few threads, or tie by the hundred
+        __syncthreads();  // every thread has read n
+        top_scan(R, A.top_n, *top);
+      } else {
+        sort_runs(*top, n);
+      }
+      bad = !(tp.s >= 0.0);
       if (bad) {
         for (int i = tid; i < A.top_n; i += kRowThreads) put(i, 0);
-      } else if (n <= kRank) {
-        // a key's place is the number of larger ones
-        for (int i = tid; i < n; i += kRowThreads) {
-          const unsigned long long k = top->key[i];
-          int place = 0;
-#pragma unroll 8
-          for (int j = 0; j < n; j++) place += top->key[j] > k;
-          if (place < A.top_n) put(place, k);
-        }
-        for (int i = n + tid; i < A.top_n; i += kRowThreads) put(i, 0);
-      } else {
-        if (n <= kBuf) {
-          for (int i = n + tid; i < kBuf; i += kRowThreads) top->key[i] = 0;
-          sort_desc(top->key, kBuf);
-        } else {  // rows whose largest elements crowd into few threads, or tie by the hundred
-          __syncthreads();  // every thread has read n
-          top_scan(R, A.top_n, *top);
-        }
+      } else if (n > kBuf) {
         for (int i = tid; i < A.top_n; i += kRowThreads) put(i, top->key[i]);
+      } else {
+        place_keys(*top, n, A.top_n, put);
       }
       __syncthreads();  // before the next row's keys
     }
@@ -1010,19 +1147,17 @@ __device__ __forceinline__ void zero_slice(const Row<T>& R, const Slice<T>& S, T
   if (S.edge >= 0) d[S.edge] = from_f<T>(0.f);
 }
 
-// 2 CTAs an SM; a slice of up to 96 KiB stays in its threads' rings.
-constexpr int kDistillCtas = 2, kDistillDepth = 6;
+constexpr int kDistillCtas = 3, kDistillDepth = 4;
 constexpr int kDistillRing = kDistillDepth * kBatch * kRowThreads * 16;
 
 // A cluster's rows, one after the other.  The teacher's list (thread j holds
 // entry j) is every CTA's; the sums are over the ids that are not listed, so
 // that the mass outside the list is a sum of its own and no difference of two
 // near 1; the listed ids come out of the vectors as they are read, each thread
-// following the chain of those that its vectors hold.  The gradient is a
-// second pass over the slice: over the ring, which holds the whole slice (KEEP)
-// and takes in the next row's step for each one that is written, or out of L2
-// where a slice is larger.
-template <typename T, bool KEEP>
+// following the chain of those that its vectors hold.  The gradient (GRAD) is
+// a second pass over the slice, out of L2 and through the same rings, whose
+// copies start before the sums are joined.
+template <typename T, bool GRAD>
 __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(DistillArgs A) {
   static_assert(kScoreMax <= kRowThreads, "one list entry a thread");
   extern __shared__ uint4 ring[];
@@ -1034,15 +1169,16 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = A.K;
   const bool logits = A.kind == MS_TEACHER_LOGITS;
   const int64_t begin = blockIdx.x / ranks, stride = gridDim.x / ranks;
-  Feed<T, kDistillDepth> feed;
+  Feed<T, kDistillDepth, GRAD> feed;
   feed.rows = {A.ids, A.loss ? nullptr : A.weight, K, A.V, A.B, stride, -1, 1.f};
   feed.x = A.x;
   feed.ld = A.ld;
   feed.rank = rank;
   feed.ranks = ranks;
-  feed.ring = smem_addr(ring + tid);
-  feed.start(begin);
-  int slot = 0, which = 0, joined = 0, turn = 0;
+  Place<kDistillDepth> place(smem_addr(ring + tid));
+  feed.rows.fetch(begin);
+  feed.start(begin, place);
+  int which = 0, joined = 0, turn = 0;
   int id_in = -1;  // thread j's entry of the row after the next prepared one, and its weight
   float val_in = -INFINITY, w_in = 1.f;
   auto fetch = [&](int64_t r) {
@@ -1082,7 +1218,9 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
     const Slice<T> S(R, rank, ranks);
     T* d = (T*)A.dx + r * A.dld;
     const bool same = (((uintptr_t)d ^ (uintptr_t)R.p) & 15) == 0;
-    const int steps = S.steps(), last = S.last();
+    int rest_vecs;  // of the step after the thread's whole ones
+    const int whole = S.whole_steps(&rest_vecs);
+    const bool part = whole < S.steps();
     DistillList& L = list[which];
     DistillJoin& J = join[joined];
     const float w = w_next, val = val_next;
@@ -1121,20 +1259,32 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
       return next;
     };
     int next = next_from(S.w0);
-    const int slot0 = slot;
-    for (int k = 0, v = S.w0 + tid; k < steps; k++, v += STEP) {
-      // KEEP: no copies start in this pass, so fewer and fewer are in flight behind the step's
-      if (KEEP) copies_wait<kDistillDepth - 1>(kDistillDepth - 1 - k);
-      else copies_wait<kDistillDepth - 1>();
+    int v = S.w0 + tid;
+#pragma unroll 1
+    for (int k = 0; k < whole; k++, v += STEP) {
+      copies_wait<kDistillDepth - 1>();
       uint32_t x[4 * kBatch];
-      ring_step<T>(ring + slot * STEP + tid, k + 1 < steps ? kBatch : last, x);
-      slot = slot + 1 == kDistillDepth ? 0 : slot + 1;
+      ring_step(place.at, x);
       if (next < v + STEP) {
         for (int j = head; j >= 0; j = L.link[j]) mask_element<T>(x, L.id[j] + R.mis - v * VEC);
         next = next_from(v + STEP);
       }
       add_words<T, 4 * kBatch, false>(t, x, A.a);
-      if (!KEEP) feed.next();
+      feed.next(place.at);
+      place.next();
+    }
+    if (part) {
+      copies_wait<kDistillDepth - 1>();
+#pragma unroll 1
+      for (int i = 0; i < rest_vecs; i++) {
+        const uint4 u = ring_vec(place.at + i * (kRowThreads * 16));
+        uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        if (next < INT_MAX)
+          for (int j = head; j >= 0; j = L.link[j]) mask_element<T>(x, L.id[j] + R.mis - (v + i * kRowThreads) * VEC);
+        add_words<T, 4, false>(t, x, A.a);
+      }
+      feed.next(place.at);
+      place.next();
     }
     if (S.edge >= 0) {
       bool listed = false;
@@ -1163,7 +1313,8 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
 
     // ---- the row's sums
     if (warp == 0) {
-      const RowSums o = join_warps<false>(J.warp, A.a), l = join_warps<false>(J.warp_listed, A.a);
+      const RowSums o = join_warps<false>(kRowWarps, A.a, [&](int i) { return J.warp[i]; });
+      const RowSums l = join_warps<false>(kRowWarps, A.a, [&](int i) { return J.warp_listed[i]; });
       if (lane == 0) {
         J.others = o;
         J.listed = l;
@@ -1243,11 +1394,12 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
     if (!isinf(zo)) cd *= exp_small(((double)zo - (double)mo * (double)A.a) * 0.693147180559945309417);
     const float c = (float)cd;
     auto term = [&](float x) { return c * ex2_approx(isinf(zo) ? __fsub_rn(x, mo) * A.a : fmaf(x, A.a, -zo)); };
-    auto put = [&](int v, const uint4& u) {
+    const bool plain = same && !isinf(zo);
+    const f32x2 a2 = f2_pack(A.a, A.a), z2 = f2_pack(-zo, -zo), c2 = f2_pack(c, c);
+    auto put = [&](int w, const uint4& u) {  // vector w of the row
       float f[VEC];
-      if (!isinf(zo)) {
+      if (plain) {
         const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-        const f32x2 a2 = f2_pack(A.a, A.a), z2 = f2_pack(-zo, -zo), c2 = f2_pack(c, c);
         constexpr int PER = VEC / 4, WORDS = 2 / PER;  // elements a word, words a pair
 #pragma unroll
         for (int i = 0; i < 4; i += WORDS) {
@@ -1256,31 +1408,34 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
           f[i * PER] = e.x;
           f[i * PER + 1] = e.y;
         }
+        *reinterpret_cast<uint4*>(d + ((int64_t)w * VEC - R.mis)) = pack(f, T());
       } else {
         unpack(u, f, T());
 #pragma unroll
         for (int j = 0; j < VEC; j++) f[j] = term(f[j]);
+        store_vec(R, d, same, w, f);
       }
-      if (same) *reinterpret_cast<uint4*>(d + (v * VEC - R.mis)) = pack(f, T());
-      else store_vec(R, d, false, v, f);
     };
-    if (KEEP) {
-      slot = slot0;
-      for (int k = 0, v = S.w0 + tid; k < steps; k++, v += STEP) {
-        if (pass) {
-          const uint4* src = ring + slot * STEP + tid;
-          const int n = k + 1 < steps ? kBatch : last;
-#pragma unroll
-          for (int i = 0; i < kBatch; i++)
-            if (i < n) put(v + i * kRowThreads, src[i * kRowThreads]);
-        }
-        slot = slot + 1 == kDistillDepth ? 0 : slot + 1;
-        feed.next();
+    if (GRAD) {  // from the last step to the first
+      if (part) {
+        copies_wait<kDistillDepth - 1>();
+        if (pass)
+#pragma unroll 1
+          for (int i = 0; i < rest_vecs; i++) put(v + i * kRowThreads, ring_vec(place.at + i * (kRowThreads * 16)));
+        feed.next(place.at);
+        place.next();
       }
-    } else if (pass) {
-      const uint4* src = reinterpret_cast<const uint4*>(R.p - R.mis);
-#pragma unroll 4
-      for (int v = S.w0 + tid; v < S.w1; v += kRowThreads) put(v, src[v]);
+#pragma unroll 1
+      for (int k = 0; k < whole; k++) {
+        v -= STEP;
+        copies_wait<kDistillDepth - 1>();
+        if (pass) {
+#pragma unroll
+          for (int i = 0; i < kBatch; i++) put(v + i * kRowThreads, ring_vec(place.at + i * (kRowThreads * 16)));
+        }
+        feed.next(place.at);
+        place.next();
+      }
     }
     if (pass) {
       if (S.edge >= 0) d[S.edge] = from_f<T>(term(xe));
@@ -1429,13 +1584,8 @@ cudaError_t launch_logprobs_backward(const ScoreArgs& A, int dtype, cudaStream_t
 cudaError_t launch_distill(const DistillArgs& A, int dtype, cudaStream_t stream) {
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    // a vector more than V / VEC, as a row may start anywhere in its first
-    const int64_t vecs = ((int64_t)A.V + 2 * Row<T>::VEC - 2) / Row<T>::VEC, held = kDistillRing / 16;
-    int fit = 1;
-    while (fit < kMaxCluster && (vecs + fit - 1) / fit > held) fit++;
-    const bool keep = A.dx && (vecs + fit - 1) / fit <= held;
-    if (!A.dx) fit = 1;
-    return launch_rows(keep ? distill_kernel<T, true> : distill_kernel<T, false>, A, (int64_t)A.V * sizeof(T), fit,
+    // the same CTAs a row with and without the gradient: the loss is the same to the bit
+    return launch_rows(A.dx ? distill_kernel<T, true> : distill_kernel<T, false>, A, (int64_t)A.V * sizeof(T) * 2, 1,
                        kDistillRing, stream);
   });
 }
