@@ -24,9 +24,9 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <deque>
 #include <mutex>
 #include <type_traits>
-#include <vector>
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -761,7 +761,7 @@ __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
 
 // ---------------------------------------------------------------- forward
 // 3 CTAs an SM: their rings hold 192 KiB in flight.
-constexpr int kScoreCtas = 3, kScoreDepth = 4;
+constexpr int kScoreCtas = 3, kScoreDepth = 2;
 constexpr int kScoreRing = kScoreDepth * kBatch * kRowThreads * 16;
 
 // A row's sums while they are joined, for a row and the next: the warps', and
@@ -1147,8 +1147,11 @@ __device__ __forceinline__ void zero_slice(const Row<T>& R, const Slice<T>& S, T
   if (S.edge >= 0) d[S.edge] = from_f<T>(0.f);
 }
 
-constexpr int kDistillCtas = 3, kDistillDepth = 4;
-constexpr int kDistillRing = kDistillDepth * kBatch * kRowThreads * 16;
+// CTAs an SM, and steps of their rings; the gradient's second loop takes the registers of a third CTA.
+template <bool GRAD>
+struct DistillShape {
+  static constexpr int kCtas = GRAD ? 2 : 3, kDepth = GRAD ? 3 : 2, kRing = kDepth * kBatch * kRowThreads * 16;
+};
 
 // A cluster's rows, one after the other.  The teacher's list (thread j holds
 // entry j) is every CTA's; the sums are over the ids that are not listed, so
@@ -1158,24 +1161,24 @@ constexpr int kDistillRing = kDistillDepth * kBatch * kRowThreads * 16;
 // a second pass over the slice, out of L2 and through the same rings, whose
 // copies start before the sums are joined.
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(DistillArgs A) {
+__global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distill_kernel(DistillArgs A) {
   static_assert(kScoreMax <= kRowThreads, "one list entry a thread");
   extern __shared__ uint4 ring[];
   __shared__ DistillList list[2];  // a row's and the next's
   __shared__ DistillJoin join[2];
-  constexpr int VEC = Row<T>::VEC, STEP = kBatch * kRowThreads;
+  constexpr int VEC = Row<T>::VEC, STEP = kBatch * kRowThreads, kDepth = DistillShape<GRAD>::kDepth;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), ranks = (int)cl.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = A.K;
   const bool logits = A.kind == MS_TEACHER_LOGITS;
   const int64_t begin = blockIdx.x / ranks, stride = gridDim.x / ranks;
-  Feed<T, kDistillDepth, GRAD> feed;
+  Feed<T, kDepth, GRAD> feed;
   feed.rows = {A.ids, A.loss ? nullptr : A.weight, K, A.V, A.B, stride, -1, 1.f};
   feed.x = A.x;
   feed.ld = A.ld;
   feed.rank = rank;
   feed.ranks = ranks;
-  Place<kDistillDepth> place(smem_addr(ring + tid));
+  Place<kDepth> place(smem_addr(ring + tid));
   feed.rows.fetch(begin);
   feed.start(begin, place);
   int which = 0, joined = 0, turn = 0;
@@ -1262,7 +1265,7 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
     int v = S.w0 + tid;
 #pragma unroll 1
     for (int k = 0; k < whole; k++, v += STEP) {
-      copies_wait<kDistillDepth - 1>();
+      copies_wait<kDepth - 1>();
       uint32_t x[4 * kBatch];
       ring_step(place.at, x);
       if (next < v + STEP) {
@@ -1274,7 +1277,7 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
       place.next();
     }
     if (part) {
-      copies_wait<kDistillDepth - 1>();
+      copies_wait<kDepth - 1>();
 #pragma unroll 1
       for (int i = 0; i < rest_vecs; i++) {
         const uint4 u = ring_vec(place.at + i * (kRowThreads * 16));
@@ -1326,19 +1329,21 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
     double Q = 0.0, log_top = 0.0;  // the teacher's mass; for logits, its log relative to the largest
     float top = 0.f;
     bool live = true;               // some entry is present
+    const double mass_in = lane < kRowWarps ? L.mass[lane] : 0.0;
     if (logits) {
-      top = -INFINITY;
+      const float m_in = lane < kRowWarps ? L.m[lane] : -INFINITY;
+      top = warp_max_f(m_in);
+      Q = mass_in == 0.0 ? 0.0 : mass_in * exp(((double)m_in - (double)top) * A.rT);
+    } else {
+      Q = mass_in;
+    }
 #pragma unroll
-      for (int i = 0; i < kRowWarps; i++) top = fmaxf(top, L.m[i]);
-#pragma unroll
-      for (int i = 0; i < kRowWarps; i++)
-        if (L.mass[i] != 0.0) Q += L.mass[i] * exp(((double)L.m[i] - (double)top) * A.rT);
+    for (int o = kRowWarps / 2; o > 0; o >>= 1) Q += __shfl_xor_sync(0xffffffffu, Q, o);
+    Q = __shfl_sync(0xffffffffu, Q, 0);
+    if (logits) {
       live = Q != 0.0;
       log_top = log(Q);
       Q = Q == Q ? 1.0 : Q;
-    } else {
-#pragma unroll
-      for (int i = 0; i < kRowWarps; i++) Q += L.mass[i];
     }
     double rest = logits ? 0.0 : 1.0 - Q;
     if (rest < kNoTail) rest = 0.0;
@@ -1396,42 +1401,48 @@ __global__ void __launch_bounds__(kRowThreads, kDistillCtas) distill_kernel(Dist
     auto term = [&](float x) { return c * ex2_approx(isinf(zo) ? __fsub_rn(x, mo) * A.a : fmaf(x, A.a, -zo)); };
     const bool plain = same && !isinf(zo);
     const f32x2 a2 = f2_pack(A.a, A.a), z2 = f2_pack(-zo, -zo), c2 = f2_pack(c, c);
-    auto put = [&](int w, const uint4& u) {  // vector w of the row
-      float f[VEC];
-      if (plain) {
-        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-        constexpr int PER = VEC / 4, WORDS = 2 / PER;  // elements a word, words a pair
-#pragma unroll
-        for (int i = 0; i < 4; i += WORDS) {
-          const float2 y = f2_unpack(f2_fma(pair_of(x[i], x[i + WORDS - 1], T()), a2, z2));
-          const float2 e = f2_unpack(f2_mul(f2_pack(ex2_approx(y.x), ex2_approx(y.y)), c2));
-          f[i * PER] = e.x;
-          f[i * PER + 1] = e.y;
-        }
-        *reinterpret_cast<uint4*>(d + ((int64_t)w * VEC - R.mis)) = pack(f, T());
-      } else {
-        unpack(u, f, T());
+    // n of the step's vectors, the first being the row's v
+    auto put = [&](int v, uint32_t at, int n) {
+#pragma unroll 1
+      for (int i = 0; i < n; i++) {
+        float f[VEC];
+        unpack(ring_vec(at + i * (kRowThreads * 16)), f, T());
 #pragma unroll
         for (int j = 0; j < VEC; j++) f[j] = term(f[j]);
-        store_vec(R, d, same, w, f);
+        store_vec(R, d, same, v + i * kRowThreads, f);
       }
     };
     if (GRAD) {  // from the last step to the first
       if (part) {
-        copies_wait<kDistillDepth - 1>();
-        if (pass)
-#pragma unroll 1
-          for (int i = 0; i < rest_vecs; i++) put(v + i * kRowThreads, ring_vec(place.at + i * (kRowThreads * 16)));
+        copies_wait<kDepth - 1>();
+        if (pass) put(v, place.at, rest_vecs);
         feed.next(place.at);
         place.next();
       }
+      uint4* to = reinterpret_cast<uint4*>(d - R.mis) + v;  // a 16-byte boundary where `same`
 #pragma unroll 1
       for (int k = 0; k < whole; k++) {
         v -= STEP;
-        copies_wait<kDistillDepth - 1>();
-        if (pass) {
+        to -= STEP;
+        copies_wait<kDepth - 1>();
+        if (pass && plain) {
 #pragma unroll
-          for (int i = 0; i < kBatch; i++) put(v + i * kRowThreads, ring_vec(place.at + i * (kRowThreads * 16)));
+          for (int i = 0; i < kBatch; i++) {
+            constexpr int PER = VEC / 4, WORDS = 2 / PER;  // elements a word, words a pair
+            const uint4 u = ring_vec(place.at + i * (kRowThreads * 16));
+            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+            float f[VEC];
+#pragma unroll
+            for (int j = 0; j < 4; j += WORDS) {
+              const float2 y = f2_unpack(f2_fma(pair_of(x[j], x[j + WORDS - 1], T()), a2, z2));
+              const float2 e = f2_unpack(f2_mul(f2_pack(ex2_approx(y.x), ex2_approx(y.y)), c2));
+              f[j * PER] = e.x;
+              f[j * PER + 1] = e.y;
+            }
+            to[i * kRowThreads] = pack(f, T());
+          }
+        } else if (pass) {
+          put(v, place.at, kBatch);
         }
         feed.next(place.at);
         place.next();
@@ -1483,27 +1494,27 @@ cudaLaunchConfig_t row_config(int ranks, int64_t ctas, int ring, cudaStream_t st
   return cfg;
 }
 
-// A kernel's row clusters: how many of each size the current device runs at
+// A row kernel's clusters: how many of each size the current device runs at
 // once (0: none), asked of the driver once.  A grid of that many clusters has
 // no second wave, which would cost as much as the first.
+struct RowClusters {
+  const void* kernel;
+  int device, n[kMaxCluster + 1];
+};
 template <typename Args>
-cudaError_t row_clusters(void (*kernel)(Args), int ring, int ranks, int* clusters) {
-  struct Known {
-    void (*kernel)(Args);
-    int device, n[kMaxCluster + 1];
-  };
+cudaError_t row_clusters(void (*kernel)(Args), int ring, const RowClusters** found) {
   static std::mutex mu;
-  static std::vector<Known> known;
+  static std::deque<RowClusters> known;  // its elements stay where they are
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
   std::lock_guard<std::mutex> lock(mu);
-  for (const Known& k : known)
-    if (k.kernel == kernel && k.device == device) {
-      *clusters = k.n[ranks];
+  for (const RowClusters& k : known)
+    if (k.kernel == (const void*)kernel && k.device == device) {
+      *found = &k;
       return cudaSuccess;
     }
-  Known k = {kernel, device, {}};
+  RowClusters k = {(const void*)kernel, device, {}};
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring);
   // clusters beyond the portable size
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -1519,34 +1530,36 @@ cudaError_t row_clusters(void (*kernel)(Args), int ring, int ranks, int* cluster
   }
   if (e != cudaSuccess) return e;
   known.push_back(k);
-  *clusters = k.n[ranks];
+  *found = &known.back();
   return cudaSuccess;
 }
 
-// Launches a row kernel with the best CTAs a row, `fit` or more.  The rows go
-// over the clusters in rounds, so the time is about rounds * (slice + what a
-// row costs its CTAs beside the copies), in bytes at a CTA's share of the
-// bandwidth.
-template <typename Args>
-cudaError_t launch_rows(void (*kernel)(Args), const Args& A, int64_t row_bytes, int fit, int ring,
-                        cudaStream_t stream) {
-  int best = 0, best_clusters = 0;
+// The best CTAs a row, `fit` or more, from a kernel's clusters.  The rows go over
+// the clusters in rounds, so the time is about rounds * (slice + what a row
+// costs its CTAs beside the copies), in bytes at a CTA's share of the
+// bandwidth: `one` for a CTA by itself, `joined` where CTAs meet, and 2 KiB for
+// each of them.
+int best_ranks(const RowClusters& k, int64_t B, int64_t row_bytes, int fit, int64_t one, int64_t joined) {
+  int best = 0;
   int64_t least = INT64_MAX;
   for (int c = fit; c <= kMaxCluster; c++) {
-    int n = 0;
-    const cudaError_t e = row_clusters(kernel, ring, c, &n);
-    if (e != cudaSuccess) return e;
+    const int n = k.n[c];
     if (n < 1) continue;
-    const int64_t cost = (A.B + n - 1) / n * (row_bytes / c + (c == 1 ? 16384 : 24576 + 2048 * c));
+    const int64_t cost = (B + n - 1) / n * (row_bytes / c + (c == 1 ? one : joined + 2048 * c));
     if (cost < least) {
       least = cost;
       best = c;
-      best_clusters = n;
     }
   }
-  if (best == 0) return cudaErrorInvalidConfiguration;
+  return best;
+}
+
+template <typename Args>
+cudaError_t launch_rows(void (*kernel)(Args), const Args& A, const RowClusters& k, int ranks, int ring,
+                        cudaStream_t stream) {
+  if (ranks < 1 || k.n[ranks] < 1) return cudaErrorInvalidConfiguration;
   cudaLaunchAttribute at;
-  const cudaLaunchConfig_t cfg = row_config(best, std::min<int64_t>(A.B, best_clusters) * best, ring, stream, &at);
+  const cudaLaunchConfig_t cfg = row_config(ranks, std::min<int64_t>(A.B, k.n[ranks]) * ranks, ring, stream, &at);
   return cudaLaunchKernelEx(&cfg, kernel, A);
 }
 
@@ -1560,7 +1573,11 @@ cudaError_t launch_logprobs(const ScoreArgs& A, int dtype, cudaStream_t stream) 
                  : (top ? logprobs_kernel<T, false, true> : logprobs_kernel<T, false, false>);
     // the bounds want twice as many threads a row as alternatives
     const int fit = A.top_n > kRowThreads / 2 ? 2 : 1;
-    return launch_rows(k, A, (int64_t)A.V * sizeof(T), fit, kScoreRing, stream);
+    const RowClusters* rc = nullptr;
+    const cudaError_t e = row_clusters(k, kScoreRing, &rc);
+    if (e != cudaSuccess) return e;
+    const int ranks = best_ranks(*rc, A.B, (int64_t)A.V * sizeof(T), fit, 16384, top ? 32768 : 24576);
+    return launch_rows(k, A, *rc, ranks, kScoreRing, stream);
   });
 }
 
@@ -1585,8 +1602,14 @@ cudaError_t launch_distill(const DistillArgs& A, int dtype, cudaStream_t stream)
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     // the same CTAs a row with and without the gradient: the loss is the same to the bit
-    return launch_rows(A.dx ? distill_kernel<T, true> : distill_kernel<T, false>, A, (int64_t)A.V * sizeof(T) * 2, 1,
-                       kDistillRing, stream);
+    const RowClusters* rc = nullptr;
+    cudaError_t e = row_clusters(distill_kernel<T, true>, DistillShape<true>::kRing, &rc);
+    if (e != cudaSuccess) return e;
+    const int ranks = best_ranks(*rc, A.B, (int64_t)A.V * sizeof(T) * 2, 1, 65536, 131072);
+    if (A.dx) return launch_rows(distill_kernel<T, true>, A, *rc, ranks, DistillShape<true>::kRing, stream);
+    e = row_clusters(distill_kernel<T, false>, DistillShape<false>::kRing, &rc);
+    if (e != cudaSuccess) return e;
+    return launch_rows(distill_kernel<T, false>, A, *rc, ranks, DistillShape<false>::kRing, stream);
   });
 }
 

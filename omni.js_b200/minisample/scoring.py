@@ -37,20 +37,23 @@ def _block(s, x, what="logits"):
     if dtype is None or x.dim() != 2:
         raise ValueError(f"{what} must be a [B, V] float32, bfloat16 or float16 CUDA tensor")
     B, V = x.shape
-    if V > 1 and x.stride(1) != 1:
+    ld, col = x.stride()
+    if col != 1 and V > 1:
         raise ValueError(f"{what} must have unit column stride")
-    if B > 1 and x.stride(0) < V:
+    if B <= 1:
+        ld = V
+    elif ld < V:
         raise ValueError(f"{what} must have a row stride of at least V (an expanded block has its rows on one another)")
-    if x.device.index != s.device_index:
-        raise ValueError(f"{what} is on cuda:{x.device.index}, the sampler on cuda:{s.device_index}")
-    return dtype, B, V, (x.stride(0) if B > 1 else V)
+    if x.get_device() != s.device_index:
+        raise ValueError(f"{what} is on cuda:{x.get_device()}, the sampler on cuda:{s.device_index}")
+    return dtype, B, V, ld
 
 
 def _rows(t, name, x, dtype, shape):
     """Checks a small per-row argument: type, shape, device; contiguous."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != x.device:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != x.get_device():
         raise ValueError(f"{name} must be a {dtype} tensor on {x.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -59,8 +62,7 @@ def _tokens(tokens, x):
     """(contiguous tokens or None, their number a row)."""
     if tokens is None:
         return None, 0
-    B = x.shape[0]
-    if not isinstance(tokens, torch.Tensor) or tokens.dim() not in (1, 2) or tokens.shape[0] != B:
+    if not isinstance(tokens, torch.Tensor) or tokens.dim() not in (1, 2) or tokens.shape[0] != x.shape[0]:
         raise ValueError("tokens must be a [B] or [B, n] int32 tensor")
     n = 1 if tokens.dim() == 1 else tokens.shape[1]
     if n == 0:
@@ -92,9 +94,14 @@ def _on(stream, tensors, call):
     return r
 
 
-def _current(x):
+# the current stream's handle without the Stream object around it, where torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _current(s):
     # handle 0 is the legacy default stream, which the C ABI knows as 1
-    return torch.cuda.current_stream(x.device).cuda_stream or 1
+    return _raw_stream(s.device_index) or 1
 
 
 # ---------------------------------------------------------------- log-probabilities
@@ -112,7 +119,7 @@ def _logprobs(s, x, tokens, temperature, top_n, entropy, stats):
     sm = torch.empty(B, dtype=torch.float64, device=dev) if stats else None
     out = N.MsScores(_p(lp), _p(ent), _p(ids), _p(top), _p(mx), _p(sm))
     s._check(s._L.ms_logprobs(s._ctx, x.data_ptr(), dtype, B, V, ld, temperature, _p(tok), n, top_n,
-                              ctypes.byref(out), _current(x)))
+                              ctypes.byref(out), _current(s)))
     return LogProbs(lp, ent, ids, top, mx, sm)
 
 
@@ -167,7 +174,7 @@ def logprobs_backward(s, logits, tokens, row_max, row_sum, g_logprobs=None, g_en
     dx = _grad_out(s, logits, out)
     s._check(s._L.ms_logprobs_backward(s._ctx, logits.data_ptr(), dtype, B, V, ld, temperature, _p(tok), n,
                                        row_max.data_ptr(), row_sum.data_ptr(), _p(entropy), _p(g_logprobs),
-                                       _p(g_entropy), dx.data_ptr(), dx.stride(0), _current(logits)))
+                                       _p(g_entropy), dx.data_ptr(), dx.stride(0), _current(s)))
     return dx
 
 
@@ -186,7 +193,7 @@ def _distill(s, x, ids, values, weight, temperature, kind, want_loss, dx):
     loss = torch.empty(B, dtype=torch.float32, device=x.device) if want_loss else None
     s._check(s._L.ms_distill(s._ctx, x.data_ptr(), dtype, B, V, ld, temperature, ids.data_ptr(), values.data_ptr(), K,
                              _KINDS[kind], _p(weight), _p(loss), _p(dx), dx.stride(0) if dx is not None else 0,
-                             _current(x)))
+                             _current(s)))
     return loss
 
 
