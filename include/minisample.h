@@ -186,7 +186,8 @@ int ms_profile_read(ms_ctx* ctx, double* stream_ms, double* finalize_ms, int64_t
  * rows), one when greedy or for top-k calls of at most 16 rows, two for
  * larger top-k calls (the chunk kernel and the row finalize), four for
  * whole-vocabulary rows (chunk kernel, plan, extract,
- * resolve); one per ms_history_append.  No reference counterpart.
+ * resolve); one per ms_history_append; one per scoring call (ms_logprobs,
+ * ms_logprobs_backward, ms_distill).  No reference counterpart.
  */
 int ms_launch_count(ms_ctx* ctx, int64_t* kernels);
 
@@ -363,8 +364,8 @@ int ms_logprobs(ms_ctx* ctx, const void* logits, int dtype, int64_t B, int64_t V
  *            tokens and temperature
  *   g_logprobs  [B, n_tokens] or NULL (0); read only where the token is one
  *   g_entropy   [B] or NULL (0); needs entropy [B] (NULL without it)
- *   dlogits  [B, dld] of `dtype`, dld >= V; may be `logits` itself (dld = ld),
- *            and must not overlap it otherwise
+ *   dlogits  [B, dld] of `dtype`, dld >= V; may be `logits` itself (dld = ld);
+ *            otherwise the two blocks' address ranges must not overlap
  * Padding rows, rows of -Inf alone and rows whose gradients are all 0 get 0.
  */
 int ms_logprobs_backward(ms_ctx* ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t ld,

@@ -7,8 +7,8 @@
 //   H          = log s - (1/s) sum exp(z - m) (z - m)
 // so one pass over the row with a running maximum (m, s and the sum of
 // exp(z - m)(z - m), rescaled when the maximum moves) gives everything but the
-// alternatives.  Each thread keeps its own running maximum and fp32 sums of at
-// most a few hundred terms; threads are combined in fp64.
+// alternatives.  Each thread keeps its own running maximum and fp32 sums (of a
+// step's terms, then of the steps); warps are joined in fp64.
 //
 // A row is one thread-block cluster's: its CTAs take equal slices and exchange
 // their sums (a few numbers) through distributed shared memory, so a call needs
@@ -24,7 +24,6 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
-#include <deque>
 #include <mutex>
 #include <type_traits>
 
@@ -41,7 +40,9 @@ namespace {
 
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kBatch = 4;       // 16-byte vectors of a thread's step
+// 16-byte vectors of a thread's step.  2 instead, with twice the steps in flight
+// (same bytes): 2048 x 151936 bf16 103 -> 114 us, distillation of 4096 rows 537 -> 556 us.
+constexpr int kBatch = 4;
 constexpr int kMaxCluster = 16;
 constexpr int kBuf = 992;       // keys the selection holds (runs of 32)
 constexpr int kScan = 512;      // of them, those that the tiled selection uses: top_n and a tile of kRowThreads
@@ -236,16 +237,18 @@ __device__ __forceinline__ void add_words(Sums& t, const uint32_t (&w)[N], float
   constexpr int PER = sizeof(T) == 4 ? 2 : 1;  // words a pair
   const float hi = largest(w, T());
   if (hi > t.m) raise_to<ENT>(t, hi, a);
+  // The words' own sum first, then onto the thread's: its roundings grow with
+  // the thread's steps and not with its elements.
   if (!t.odd) {
     const f32x2 z2 = f2_pack(-t.z, -t.z), a2 = f2_pack(a, a);
-    f32x2 s = t.s, q = t.q;
+    f32x2 s = 0, q = 0;
 #pragma unroll
     for (int i = 0; i < N; i += PER) {
       const f32x2 y2 = f2_fma(pair_of(w[i], w[i + PER - 1], T()), a2, z2);
       const float2 y = f2_unpack(y2);
       const f32x2 e = f2_pack(ex2_approx(y.x), ex2_approx(y.y));
-      s = f2_add(s, e);
-      if constexpr (ENT) q = f2_fma(e, y2, q);
+      s = i == 0 ? e : f2_add(s, e);
+      if constexpr (ENT) q = i == 0 ? f2_mul(e, y2) : f2_fma(e, y2, q);
     }
     t.odd = isinf(t.z);
     if constexpr (ENT) {
@@ -253,21 +256,24 @@ __device__ __forceinline__ void add_words(Sums& t, const uint32_t (&w)[N], float
       t.odd |= isnan(h.x + h.y);
     }
     if (!t.odd) {
-      t.s = s;
-      t.q = q;
+      t.s = f2_add(t.s, s);
+      if constexpr (ENT) t.q = f2_add(t.q, q);
       return;
     }
   }
   const float m = t.m == -INFINITY ? 0.f : t.m;
+  f32x2 s = 0, q = 0;
 #pragma unroll
   for (int i = 0; i < N; i += PER) {
     const float2 x = f2_unpack(pair_of(w[i], w[i + PER - 1], T()));
     const float y0 = bounded(isinf(t.z) ? __fsub_rn(x.x, m) * a : fmaf(x.x, a, -t.z));
     const float y1 = bounded(isinf(t.z) ? __fsub_rn(x.y, m) * a : fmaf(x.y, a, -t.z));
     const f32x2 e = f2_pack(ex2_approx(y0), ex2_approx(y1));
-    t.s = f2_add(t.s, e);
-    if constexpr (ENT) t.q = f2_fma(e, f2_pack(y0, y1), t.q);
+    s = i == 0 ? e : f2_add(s, e);
+    if constexpr (ENT) q = i == 0 ? f2_mul(e, f2_pack(y0, y1)) : f2_fma(e, f2_pack(y0, y1), q);
   }
+  t.s = f2_add(t.s, s);
+  if constexpr (ENT) t.q = f2_add(t.q, q);
 }
 
 template <bool ENT>
@@ -593,6 +599,11 @@ struct TopSmem {
   int n;
 };
 
+// Up to this many (CTAs a row) * (bounds) a CTA goes by its own bound; beyond,
+// the CTAs meet first to find the row's.  Meeting costs about 1 us of a row and
+// leaves fewer keys: one row of 50257, top 5, 7 CTAs (7): 9.9 us alone, 10.4 met;
+// 16 CTAs (16): 12.5 alone, 11.5 met; 64 x 128256 top 20, 4 CTAs (12): 20.0 alone,
+// 17.8 met; 512 x 262144 top 64, 2 CTAs (16): 199 alone, 176 met.
 constexpr int kAlone = 10;
 constexpr int kRounds = kScoreMax / kRowWarps;  // bounds that a CTA gives for the largest top_n
 
@@ -760,7 +771,11 @@ __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
 }
 
 // ---------------------------------------------------------------- forward
-// 3 CTAs an SM: their rings hold 192 KiB in flight.
+// CTAs an SM and steps of their rings: 96 KiB in flight an SM.  Every other load
+// (tokens, the alternatives' second read) waits behind what the rings have asked
+// for: with 4 steps 512 x 262144 top 64 takes 162 us instead of 139, and
+// 2048 x 151936 bf16 105 instead of 103.  4 CTAs, at 64 registers: 175 and 120 us;
+// 2 CTAs with 6 steps: 205 and 112 us.
 constexpr int kScoreCtas = 3, kScoreDepth = 2;
 constexpr int kScoreRing = kScoreDepth * kBatch * kRowThreads * 16;
 
@@ -829,7 +844,10 @@ __device__ __forceinline__ void write_row(const ScoreArgs& A, int64_t r, const R
       O.logprobs[r * A.n_tok + t] = lp;
     }
   if (lane == 0) {
-    if (ENT) O.entropy[r] = empty ? 0.f : (float)(log_s - sum.q / sum.s);
+    if (ENT) {
+      const double h = empty ? 0.0 : log_s - sum.q / sum.s;
+      O.entropy[r] = h < 0.0 ? 0.f : (float)h;  // one id left: 0 but for rounding
+    }
     if (O.row_max) O.row_max[r] = (double)sum.m / A.T;
     if (O.row_sum) O.row_sum[r] = sum.s;
   }
@@ -1147,7 +1165,10 @@ __device__ __forceinline__ void zero_slice(const Row<T>& R, const Slice<T>& S, T
   if (S.edge >= 0) d[S.edge] = from_f<T>(0.f);
 }
 
-// CTAs an SM, and steps of their rings; the gradient's second loop takes the registers of a third CTA.
+// CTAs an SM, and steps of their rings.  The gradient's second loop takes the
+// registers of a third CTA: 4096 x 151936 bf16 with gradient 537 us, with three
+// CTAs that spill 567; the loss alone, 1024 x 151936 with 256 listed ids, 100 us
+// with three, 120 with two.  Of the rings' steps: 2 580 us, 3 538, 4 546, 6 542.
 template <bool GRAD>
 struct DistillShape {
   static constexpr int kCtas = GRAD ? 2 : 3, kDepth = GRAD ? 3 : 2, kRing = kDepth * kBatch * kRowThreads * 16;
@@ -1503,18 +1524,22 @@ struct RowClusters {
 };
 template <typename Args>
 cudaError_t row_clusters(void (*kernel)(Args), int ring, const RowClusters** found) {
+  constexpr int kKnown = 512;  // kernels times devices
   static std::mutex mu;
-  static std::deque<RowClusters> known;  // its elements stay where they are
+  static RowClusters known[kKnown];
+  static int n_known = 0;
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
   std::lock_guard<std::mutex> lock(mu);
-  for (const RowClusters& k : known)
-    if (k.kernel == (const void*)kernel && k.device == device) {
-      *found = &k;
+  for (int i = 0; i < n_known; i++)
+    if (known[i].kernel == (const void*)kernel && known[i].device == device) {
+      *found = &known[i];
       return cudaSuccess;
     }
-  RowClusters k = {(const void*)kernel, device, {}};
+  if (n_known == kKnown) return cudaErrorMemoryAllocation;
+  RowClusters& k = known[n_known];
+  k = {(const void*)kernel, device, {}};
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring);
   // clusters beyond the portable size
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -1529,8 +1554,8 @@ cudaError_t row_clusters(void (*kernel)(Args), int ring, const RowClusters** fou
     }
   }
   if (e != cudaSuccess) return e;
-  known.push_back(k);
-  *found = &known.back();
+  n_known++;
+  *found = &k;
   return cudaSuccess;
 }
 
@@ -1560,7 +1585,9 @@ cudaError_t launch_rows(void (*kernel)(Args), const Args& A, const RowClusters& 
   if (ranks < 1 || k.n[ranks] < 1) return cudaErrorInvalidConfiguration;
   cudaLaunchAttribute at;
   const cudaLaunchConfig_t cfg = row_config(ranks, std::min<int64_t>(A.B, k.n[ranks]) * ranks, ring, stream, &at);
-  return cudaLaunchKernelEx(&cfg, kernel, A);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, A);
+  if (e != cudaSuccess) cudaGetLastError();  // it is returned here, not left for a later call
+  return e;
 }
 
 }  // namespace

@@ -1,6 +1,8 @@
 """minisample — B200 token sampler for mini.js (src/generation.js pickToken) behind libminisample.
 
   Sampler / SampleParams   batched sampling through the C ABI (include/minisample.h)
+  scoring                  log-probabilities, their gradient and distillation (Sampler.logprobs,
+                           logprobs_backward, distill_loss, distill_grad)
   generation               normalize_options / pick_token / generate_tokens mirroring
                            src/generation.js on the 'cuda' backend
   workloads                seeded synthetic logits of the benchmark shapes

@@ -68,6 +68,8 @@ def normalize_options(options: dict | None) -> dict:
         "repetition_penalty": _first(o.get("repetitionPenalty"), o.get("repetition_penalty"), default=1.0),
         "eos_token_id": _first(o.get("eosTokenId"), o.get("eos_token_id"), default=None),
         "on_token": o.get("onToken") or o.get("on_token") or None,
+        # generate_tokens_device only, no reference counterpart: alternatives a step (None: no log-probabilities)
+        "logprobs": o.get("logprobs"),
     }
 
 
@@ -237,10 +239,19 @@ def generate_tokens_device(model, input_ids_batch, options=None, rands=None):
     copies only the B ids back for the onToken / EOS rules, which are those of
     generate_tokens_batch (per row, src/generation.js:97-114).  Rows that
     stopped keep a slot in the batch; their ids are ignored and draw no
-    uniform.  Returns the generated ids of each row."""
+    uniform.  Returns the generated ids of each row.
+
+    With the option `logprobs` = n (0 <= n <= 256) returns (ids, scores): for
+    each generated id of each row a dict of its log-probability under the
+    model's own distribution (the logits before penalty and temperature), that
+    distribution's entropy, and the ids and log-probabilities of the n likeliest
+    tokens (Sampler.logprobs)."""
     import torch
 
     opts = normalize_options(options)
+    n_alt = opts["logprobs"]
+    if n_alt is not None and (isinstance(n_alt, bool) or not isinstance(n_alt, int) or not 0 <= n_alt <= 256):
+        raise ValueError("logprobs must be None or a number of alternatives in [0, 256]")
     B = len(input_ids_batch)
     rands = rands if rands is not None else [_random.random] * B
     on_token = opts["on_token"]
@@ -256,6 +267,7 @@ def generate_tokens_device(model, input_ids_batch, options=None, rands=None):
         H = DeviceHistory(input_ids_batch, cap, dev)
         ids_d = torch.empty(B, dtype=torch.int32, device=dev)
         generated = [[] for _ in range(B)]
+        scores = [[] for _ in range(B)]
         active = [True] * B
         for step in range(steps):
             if not any(active):
@@ -268,19 +280,26 @@ def generate_tokens_device(model, input_ids_batch, options=None, rands=None):
             hist = (H.hist.view(-1), H.off) if step > 0 else (None, None)
             s.sample(logits, params, u=u, hist=hist[0], hist_off=hist[1], out=ids_d, sync=False)
             H.append(s, ids_d)
+            if n_alt is not None:
+                o = s.logprobs(logits, ids_d, top_n=n_alt, entropy=True)
+                lp, ent = o.logprobs.tolist(), o.entropy.tolist()
+                top = [[[]] * B] * 2 if n_alt == 0 else (o.top_ids.tolist(), o.top_logprobs.tolist())
             ids = ids_d.cpu().numpy()
             for i in range(B):
                 if not active[i]:
                     continue
                 nid = int(ids[i])
                 generated[i].append(nid)
+                if n_alt is not None:
+                    scores[i].append({"logprob": lp[i], "entropy": ent[i], "top_ids": list(top[0][i]),
+                                      "top_logprobs": list(top[1][i])})
                 if on_token and on_token(i, nid, step + 1) is False:
                     active[i] = False
                 elif opts["eos_token_id"] is not None and nid == opts["eos_token_id"]:
                     active[i] = False
             if step + 1 < steps and any(active):
                 logits = model.forward_batch([int(x) for x in ids], caches)
-        return generated
+        return generated if n_alt is None else (generated, scores)
     finally:
         for c in caches:
             model.dispose_cache(c)

@@ -83,9 +83,11 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _on(stream, tensors, call):
+def _on(s, stream, tensors, call):
     """`call` on `stream`: what it allocates belongs to that stream, and what it
     reads is not reused by another one before it is done."""
+    if stream.device.index != s.device_index:
+        raise ValueError(f"stream is on {stream.device}, the sampler on cuda:{s.device_index}")
     with torch.cuda.stream(stream):
         r = call()
     for t in tensors:
@@ -118,7 +120,7 @@ def _logprobs(s, x, tokens, temperature, top_n, entropy, stats):
     mx = torch.empty(B, dtype=torch.float64, device=dev) if stats else None
     sm = torch.empty(B, dtype=torch.float64, device=dev) if stats else None
     out = N.MsScores(_p(lp), _p(ent), _p(ids), _p(top), _p(mx), _p(sm))
-    s._check(s._L.ms_logprobs(s._ctx, x.data_ptr(), dtype, B, V, ld, temperature, _p(tok), n, top_n,
+    s._check(s._L.ms_logprobs(s._ctx, x.data_ptr(), dtype, B, V, ld, float(temperature), _p(tok), n, top_n,
                               ctypes.byref(out), _current(s)))
     return LogProbs(lp, ent, ids, top, mx, sm)
 
@@ -146,10 +148,10 @@ class _LogProbsFn(torch.autograd.Function):
 
 def logprobs(s, logits, tokens=None, *, temperature=1.0, top_n=0, entropy=False, stats=False, stream=None):
     if stream is not None:
-        return _on(stream, (logits, tokens),
+        return _on(s, stream, (logits, tokens),
                    lambda: logprobs(s, logits, tokens, temperature=temperature, top_n=top_n, entropy=entropy,
                                     stats=stats))
-    if logits.requires_grad and torch.is_grad_enabled():
+    if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return LogProbs(*_LogProbsFn.apply(logits, s, tokens, temperature, top_n, entropy))
     return _logprobs(s, logits, tokens, temperature, top_n, entropy, stats)
 
@@ -157,7 +159,7 @@ def logprobs(s, logits, tokens=None, *, temperature=1.0, top_n=0, entropy=False,
 def logprobs_backward(s, logits, tokens, row_max, row_sum, g_logprobs=None, g_entropy=None, entropy=None, *,
                       temperature=1.0, out=None, stream=None):
     if stream is not None:
-        return _on(stream, (logits, tokens, row_max, row_sum, g_logprobs, g_entropy, entropy, out),
+        return _on(s, stream, (logits, tokens, row_max, row_sum, g_logprobs, g_entropy, entropy, out),
                    lambda: logprobs_backward(s, logits, tokens, row_max, row_sum, g_logprobs, g_entropy, entropy,
                                              temperature=temperature, out=out))
     dtype, B, V, ld = _block(s, logits)
@@ -172,8 +174,8 @@ def logprobs_backward(s, logits, tokens, row_max, row_sum, g_logprobs=None, g_en
         g_entropy = _rows(g_entropy, "g_entropy", logits, torch.float32, (B,))
         entropy = _rows(entropy, "entropy", logits, torch.float32, (B,))
     dx = _grad_out(s, logits, out)
-    s._check(s._L.ms_logprobs_backward(s._ctx, logits.data_ptr(), dtype, B, V, ld, temperature, _p(tok), n,
-                                       row_max.data_ptr(), row_sum.data_ptr(), _p(entropy), _p(g_logprobs),
+    s._check(s._L.ms_logprobs_backward(s._ctx, logits.data_ptr(), dtype, B, V, ld, float(temperature), _p(tok),
+                                       n,                                        row_max.data_ptr(), row_sum.data_ptr(), _p(entropy), _p(g_logprobs),
                                        _p(g_entropy), dx.data_ptr(), dx.stride(0), _current(s)))
     return dx
 
@@ -191,7 +193,8 @@ def _distill(s, x, ids, values, weight, temperature, kind, want_loss, dx):
     if weight is not None:
         weight = _rows(weight, "weight", x, torch.float32, (B,))
     loss = torch.empty(B, dtype=torch.float32, device=x.device) if want_loss else None
-    s._check(s._L.ms_distill(s._ctx, x.data_ptr(), dtype, B, V, ld, temperature, ids.data_ptr(), values.data_ptr(), K,
+    s._check(s._L.ms_distill(s._ctx, x.data_ptr(), dtype, B, V, ld, float(temperature), ids.data_ptr(),
+                             values.data_ptr(), K,
                              _KINDS[kind], _p(weight), _p(loss), _p(dx), dx.stride(0) if dx is not None else 0,
                              _current(s)))
     return loss
@@ -216,9 +219,9 @@ class _DistillFn(torch.autograd.Function):
 
 def distill_loss(s, logits, teacher_ids, teacher_values, *, temperature=1.0, kind="logprobs", stream=None):
     if stream is not None:
-        return _on(stream, (logits, teacher_ids, teacher_values),
+        return _on(s, stream, (logits, teacher_ids, teacher_values),
                    lambda: distill_loss(s, logits, teacher_ids, teacher_values, temperature=temperature, kind=kind))
-    if logits.requires_grad and torch.is_grad_enabled():
+    if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return _DistillFn.apply(logits, s, teacher_ids, teacher_values, temperature, kind)
     return _distill(s, logits, teacher_ids, teacher_values, None, temperature, kind, True, None)
 
@@ -226,7 +229,7 @@ def distill_loss(s, logits, teacher_ids, teacher_values, *, temperature=1.0, kin
 def distill_grad(s, logits, teacher_ids, teacher_values, weight=None, *, temperature=1.0, kind="logprobs", out=None,
                  stream=None):
     if stream is not None:
-        return _on(stream, (logits, teacher_ids, teacher_values, weight, out),
+        return _on(s, stream, (logits, teacher_ids, teacher_values, weight, out),
                    lambda: distill_grad(s, logits, teacher_ids, teacher_values, weight, temperature=temperature,
                                         kind=kind, out=out))
     _block(s, logits)

@@ -181,3 +181,13 @@ def test_oracle_distillation_gradient_against_differences(kind, T):
     loss, _, dx, _ = O.distill(x, T, ids, v, kind, 0.6, "float32")
     np.testing.assert_allclose(dx, 0.6 * _differences(f, x), atol=1e-8)
     assert loss > 0
+
+
+def test_generation_refuses_a_bad_number_of_alternatives():
+    """Before the sampler or the model is touched."""
+    from minisample.generation import generate_tokens_device, normalize_options
+
+    assert normalize_options({})["logprobs"] is None and normalize_options({"logprobs": 0})["logprobs"] == 0
+    for n in (-1, 257, 1.5, True, "5"):
+        with pytest.raises(ValueError, match="alternatives"):
+            generate_tokens_device(None, [[1]], {"logprobs": n})

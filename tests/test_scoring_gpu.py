@@ -588,7 +588,7 @@ def test_refusals(sampler):
     from minisample import MiniSampleError
 
     bad = [
-        lambda: sampler.logprobs(x.double()), lambda: sampler.logprobs(x.cpu()), lambda: sampler.logprobs(x[0]),
+        lambda: sampler.logprobs(x.cpu().numpy()), lambda: sampler.logprobs(x.double()), lambda: sampler.logprobs(x.cpu()), lambda: sampler.logprobs(x[0]),
         lambda: sampler.logprobs(x.t()), lambda: sampler.logprobs(x[:1].expand(4, 100)),
         lambda: sampler.logprobs(x[:, ::2]), lambda: sampler.logprobs(x, tok.long()),
         lambda: sampler.logprobs(x, tok[:3]), lambda: sampler.logprobs(x, tok.cpu()),
@@ -693,6 +693,41 @@ def test_captured_and_replayed(sampler):
                 assert torch.equal(a, b)
 
 
+def test_first_calls_captured():
+    """A fresh process whose first scoring calls are captured ones."""
+    code = """
+import sys
+sys.path.insert(0, %r)
+import torch
+from minisample import Sampler
+s = Sampler()
+x = torch.randn(5, 3001, device="cuda")
+tok = torch.full((5,), 7, dtype=torch.int32, device="cuda")
+g = torch.ones(5, device="cuda")
+def step():
+    o = s.logprobs(x, tok, top_n=5, entropy=True, stats=True)
+    dx = s.logprobs_backward(x, tok, o.row_max, o.row_sum, g, g, o.entropy)
+    plain = s.logprobs(x, tok)
+    return [*o, dx, plain.logprobs, *s.distill_grad(x, o.top_ids, o.top_logprobs, g),
+            s.distill_loss(x, o.top_ids, o.top_logprobs)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, step()))
+print("captured")
+"""
+    import os
+    import subprocess
+    import sys
+
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "omni.js_b200")
+    r = subprocess.run([sys.executable, "-c", code % pkg], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_results_are_the_same_every_time(sampler):
     import torch
 
@@ -749,3 +784,56 @@ def test_sampling_scoring_and_training_together(sampler):
     # a small step along the gradient moves each log-probability by its advantage's sign
     assert bool((((after.logprobs - o.logprobs) * adv) > 0).all())
     assert bool((nearer < loss).all())
+
+
+class _TableModel:
+    """forward_batch gives each row logits that depend on its last id; what it gave is kept."""
+
+    V = 5003
+
+    def __init__(self, B):
+        self.B, self.given = B, []
+
+    def make_cache(self):
+        return {}
+
+    def dispose_cache(self, cache):
+        pass
+
+    def forward_batch(self, last_ids, caches):
+        import torch
+
+        last = last_ids if last_ids is not None else list(range(self.B))
+        rows = [np.random.default_rng(1000 * len(self.given) + int(i)).normal(0, 2, self.V) for i in last]
+        self.given.append(np.stack(rows).astype(np.float32))
+        return torch.from_numpy(self.given[-1]).cuda()
+
+
+@pytest.mark.parametrize("n", [0, 4])
+def test_generation_loop_returns_log_probabilities(n):
+    """The device loop's `logprobs` option: the ids are those without it, and every generated id's scores
+    are the oracle's on the logits that the model gave."""
+    from minisample.generation import generate_tokens_device, set_backend
+
+    set_backend("cuda")
+    B = 3
+    opts = {"maxNewTokens": 5, "temperature": 0.9, "topK": 20, "topP": 0.9, "repetitionPenalty": 1.2}
+
+    def rands():
+        return [iter(np.random.default_rng(i).random(50)).__next__ for i in range(B)]
+
+    prompts = [[1, 2], [3], [4, 5, 6]]
+    plain = generate_tokens_device(_TableModel(B), prompts, opts, rands=rands())
+    eos = plain[1][2]
+    opts = dict(opts, eosTokenId=eos)
+    plain = generate_tokens_device(_TableModel(B), prompts, opts, rands=rands())
+    model = _TableModel(B)
+    ids, scores = generate_tokens_device(model, prompts, dict(opts, logprobs=n), rands=rands())
+    assert ids == plain and [len(x) for x in scores] == [len(x) for x in ids]
+    for i in range(B):
+        for step, (tok, sc) in enumerate(zip(ids[i], scores[i])):
+            want, bound = O.score(model.given[step][i], 1.0, [tok], n)
+            _near([sc["logprob"]], want["logprobs"], bound["logprobs"], (i, step))
+            _near([sc["entropy"]], [want["entropy"]], bound["entropy"], (i, step))
+            assert sc["top_ids"] == want["top_ids"].tolist()
+            _near(sc["top_logprobs"], want["top_logprobs"], bound["top_logprobs"], (i, step))
