@@ -231,9 +231,9 @@ __device__ __forceinline__ void raise_to(Sums& t, float hi, float a) {
   t.z = z;
 }
 
-// The terms of N words (N even), their maximum being in t.m already.
+// The terms of N words (N even); returns their largest element.
 template <typename T, int N, bool ENT>
-__device__ __forceinline__ void add_words(Sums& t, const uint32_t (&w)[N], float a) {
+__device__ __forceinline__ float add_words(Sums& t, const uint32_t (&w)[N], float a) {
   constexpr int PER = sizeof(T) == 4 ? 2 : 1;  // words a pair
   const float hi = largest(w, T());
   if (hi > t.m) raise_to<ENT>(t, hi, a);
@@ -258,7 +258,7 @@ __device__ __forceinline__ void add_words(Sums& t, const uint32_t (&w)[N], float
     if (!t.odd) {
       t.s = f2_add(t.s, s);
       if constexpr (ENT) t.q = f2_add(t.q, q);
-      return;
+      return hi;
     }
   }
   const float m = t.m == -INFINITY ? 0.f : t.m;
@@ -274,6 +274,7 @@ __device__ __forceinline__ void add_words(Sums& t, const uint32_t (&w)[N], float
   }
   t.s = f2_add(t.s, s);
   if constexpr (ENT) t.q = f2_add(t.q, q);
+  return hi;
 }
 
 template <bool ENT>
@@ -683,30 +684,78 @@ __device__ __forceinline__ void place_keys(const TopSmem& sh, int n, int top_n, 
   for (int i = n + threadIdx.x; i < top_n; i += kRowThreads) put(i, 0ull);
 }
 
-// Who holds a CTA's elements that reach the bound.
+// Where a thread's largest elements lie: the two steps with the largest maxima,
+// m1 >= m2, and the largest maximum m3 of the others.
+struct TopSteps {
+  float m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+  uint32_t at = 0;  // the first's step, and the second's in the upper half
+  __device__ __forceinline__ void add(float hi, int step) {
+    if (hi > m3) {
+      if (hi > m1) {
+        m3 = m2;
+        m2 = m1;
+        m1 = hi;
+        at = at << 16 | (uint32_t)step;
+      } else if (hi > m2) {
+        m3 = m2;
+        m2 = hi;
+        at = (at & 0xffffu) | (uint32_t)step << 16;
+      } else {
+        m3 = hi;
+      }
+    }
+  }
+};
+constexpr int kMostSteps = 0xffff;  // a thread's, for `at`
+
+// Who holds a CTA's elements that reach the bound: threads' steps (thread and
+// step << 8), and threads of which every step has to be read.
 struct TopOwners {
+  uint32_t step[2 * kRowThreads];
   uint8_t thread[kRowThreads];
+  int n_steps, n_threads;
 };
 
-// The CTA's elements >= bound, as keys into the buffer `to` (a peer's): only
-// threads whose maximum reaches the bound hold any, and all threads read those
-// threads' vectors again together, several in flight each.  Keys beyond the
-// buffer are counted and left out.  xe: the thread's edge element.
+// The CTA's elements >= bound, as keys into the buffer `to` (a peer's).  Only
+// steps whose maximum reaches the bound hold any; a thread knows its two
+// largest, and only where a third reaches the bound too are all of its steps
+// read.  All threads read those vectors together, out of L2 or HBM (every step
+// of those threads instead: 512 x 262144 top 64 142 us, against 129).  Keys
+// beyond the buffer are counted and left out.  xe: the thread's edge element.
 template <typename T>
-__device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, float tm, float xe, float bound,
-                                           TopOwners& own, int& owners, TopSmem* to) {
+__device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, const TopSteps& t, float xe, float bound,
+                                           TopOwners& own, TopSmem* to) {
   constexpr int VEC = Row<T>::VEC, AHEAD = 4;
+  const uint4* base = reinterpret_cast<const uint4*>(R.p - R.mis);
   auto take = [&](float x, int i) {
     if (x >= bound && x > -INFINITY) {
       const int n = atomicAdd(&to->n, 1);
       if (n < kBuf) to->key[n] = top_key(x, i);
     }
   };
-  if (tm >= bound && tm > -INFINITY) own.thread[atomicAdd(&owners, 1)] = (uint8_t)threadIdx.x;
+  auto take_vec = [&](int v, const uint4& u) {
+    float f[VEC];
+    unpack(u, f, T());
+#pragma unroll
+    for (int j = 0; j < VEC; j++) take(f[j], v * VEC - R.mis + j);
+  };
+  if (t.m3 >= bound && t.m3 > -INFINITY) {
+    own.thread[atomicAdd(&own.n_threads, 1)] = (uint8_t)threadIdx.x;
+  } else {
+    if (t.m1 >= bound && t.m1 > -INFINITY)
+      own.step[atomicAdd(&own.n_steps, 1)] = threadIdx.x | (t.at & 0xffffu) << 8;
+    if (t.m2 >= bound && t.m2 > -INFINITY)
+      own.step[atomicAdd(&own.n_steps, 1)] = threadIdx.x | (t.at >> 16) << 8;
+  }
   if (S.edge >= 0) take(xe, S.edge);
   __syncthreads();
-  const int n = owners, each = (S.w1 - S.w0 + kRowThreads - 1) / kRowThreads;
-  const uint4* base = reinterpret_cast<const uint4*>(R.p - R.mis);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < own.n_steps * kBatch; i += kRowThreads) {
+    const uint32_t o = own.step[i / kBatch];
+    const int v = S.w0 + (int)(o & 0xffu) + ((int)(o >> 8) * kBatch + i % kBatch) * kRowThreads;
+    if (v < S.w1) take_vec(v, base[v]);
+  }
+  const int n = own.n_threads, each = (S.w1 - S.w0 + kRowThreads - 1) / kRowThreads;
 #pragma unroll 1
   for (int i = threadIdx.x; i < n * each; i += AHEAD * kRowThreads) {
     uint4 u[AHEAD];
@@ -718,13 +767,8 @@ __device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, f
       if (v[a] < S.w1) u[a] = base[v[a]];
     }
 #pragma unroll
-    for (int a = 0; a < AHEAD; a++) {
-      if (v[a] >= S.w1) continue;
-      float f[VEC];
-      unpack(u[a], f, T());
-#pragma unroll
-      for (int j = 0; j < VEC; j++) take(f[j], v[a] * VEC - R.mis + j);
-    }
+    for (int a = 0; a < AHEAD; a++)
+      if (v[a] < S.w1) take_vec(v[a], u[a]);
   }
 }
 
@@ -788,11 +832,8 @@ struct ScoreJoin {
 // With alternatives: every warp's sums go to rank 0 as they are.
 struct TopJoin {
   float red[kRounds][kRowWarps];   // then in red[.][0] the bounds that the CTA tells the others
-  union {
-    float lists[4 * kRounds];      // what they all told
-    TopOwners own;
-  };
-  int owners;
+  float lists[4 * kRounds];        // what they all told
+  TopOwners own;
   float m;                         // the row's maximum and log of its sum
   double s, log_s;
   float warps[kMaxCluster * kRowWarps][3];  // every warp's {m, s, q}
@@ -908,7 +949,7 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
     const Slice<T> S(R, rank, ranks);
     const float xe = S.edge >= 0 ? to_f(R.p[S.edge]) : -INFINITY;
     if constexpr (TOP) {
-      if (tid == 0) top->n = tp.owners = 0;
+      if (tid == 0) top->n = tp.own.n_steps = tp.own.n_threads = 0;
       cluster_arrive();
     }
     // the warp that writes the row's numbers
@@ -918,25 +959,30 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
     const float xy = (uint32_t)y < (uint32_t)A.V ? to_f(R.p[y]) : 0.f;
 
     Sums t;
+    TopSteps steps;
     int rest;
     const int whole = S.whole_steps(&rest);
+    if (TOP && whole > kMostSteps) steps.m3 = INFINITY;  // a step has no number: all of them are read
 #pragma unroll 1
     for (int k = 0; k < whole; k++) {
       copies_wait<kScoreDepth - 1>();
       uint32_t w[4 * kBatch];
       ring_step(place.at, w);
-      add_words<T, 4 * kBatch, ENT>(t, w, A.a);
+      const float hi = add_words<T, 4 * kBatch, ENT>(t, w, A.a);
+      if constexpr (TOP) steps.add(hi, k);
       feed.next(place.at);
       place.next();
     }
     if (whole < S.steps()) {
       copies_wait<kScoreDepth - 1>();
+      float hi = -INFINITY;
 #pragma unroll 1
       for (int i = 0; i < rest; i++) {
         const uint4 u = ring_vec(place.at + i * (kRowThreads * 16));
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        add_words<T, 4, ENT>(t, w, A.a);
+        hi = fmaxf(hi, add_words<T, 4, ENT>(t, w, A.a));
       }
+      if constexpr (TOP) steps.add(hi, whole);
       feed.next(place.at);
       place.next();
     }
@@ -991,10 +1037,9 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
         if (tid < ranks * told) tp.lists[tid] = cl.map_shared_rank(&tp, tid / told)->red[tid % told][0];
         __syncthreads();
         bound = row_bound(tp.lists, ranks, told, rounds);
-        __syncthreads();  // the lists' place is the owners' next
       }
       if (lane < 3) cl.map_shared_rank(&tp, 0)->warps[rank * kRowWarps + warp][lane] = lane == 0 ? ws.x : lane == 1 ? ws.z : ws.w;
-      top_gather(R, S, t.m, xe, bound, tp.own, tp.owners, cl.map_shared_rank(top, 0));
+      top_gather(R, S, steps, xe, bound, tp.own, cl.map_shared_rank(top, 0));
       __syncwarp();
       cluster_arrive();
       cluster_wait();  // the gathered keys are rank 0's
