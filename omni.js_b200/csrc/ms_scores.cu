@@ -823,10 +823,10 @@ __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
 constexpr int kScoreCtas = 3, kScoreDepth = 2;
 constexpr int kScoreRing = kScoreDepth * kBatch * kRowThreads * 16;
 
-// A row's sums while they are joined, for a row and the next: the warps', and
-// the CTAs' (in the CTA that finishes the row).
+// A row's sums while they are joined: the warps', and the CTAs' (in the CTA
+// that finishes the row) for a row and the next.
 struct ScoreJoin {
-  float4 warp[2][kRowWarps];
+  float4 warp[kRowWarps][kRowWarps];  // a place for each warp whose turn it is, in a cluster two that alternate
   RowSums cta[2][kMaxCluster];
 };
 // With alternatives: every warp's sums go to rank 0 as they are.
@@ -898,8 +898,9 @@ __device__ __forceinline__ void write_row(const ScoreArgs& A, int64_t r, const R
 // slice.  Without alternatives only the warp whose turn it is waits for the
 // others: it joins the CTA's sums and hands them to the CTA whose turn it is,
 // which writes the row; both turns go round, and everyone else is at the next
-// row meanwhile (the joins are double, and a warp is never two rows ahead: it
-// passes the cluster's barrier of the row before).
+// row meanwhile.  A place of the join is free again when it is written next: by
+// itself, a CTA's warp has had its own turn since, for which the place's warp
+// had to arrive; in a cluster, it has passed the barrier of the row before.
 //
 // With alternatives, every CTA also finds bounds that top_n of its elements
 // reach, from the thread maxima that the sums need anyway.  The best bound of
@@ -921,7 +922,7 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
   const int rounds = (A.top_n + kRowWarps - 1) / kRowWarps;
   const int share = min(rounds, (2 * rounds + ranks - 1) / ranks + 2);
   // with few CTAs or alternatives each CTA's own bound leaves few enough elements
-  const bool alone = ranks * rounds <= kAlone;
+  const bool alone = ranks == 1 || ranks * rounds <= kAlone;
   const int told = alone ? rounds : share;
   const int64_t first = blockIdx.x / ranks, step = gridDim.x / ranks;
   const ms_scores& O = A.out;
@@ -936,8 +937,9 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
   Place<kScoreDepth> place(smem_addr(ring + tid));
   feed.start(first, place);
   int which = 0, turn_rank = 0, turn_warp = 0;
-  if constexpr (!TOP) cluster_arrive();
-  bool waiting = !TOP;  // for the cluster's barrier of the row before (at first: for its CTAs to have started)
+  // for the cluster's barrier of the row before (at first: for its CTAs to have started)
+  bool waiting = !TOP && ranks > 1;
+  if (waiting) cluster_arrive();
   for (int64_t r = first; r < A.B; r += step) {
     const bool live = rows.read(r);  // the same in every CTA of the cluster
     rows.fetch(r + step);
@@ -950,7 +952,7 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
     const float xe = S.edge >= 0 ? to_f(R.p[S.edge]) : -INFINITY;
     if constexpr (TOP) {
       if (tid == 0) top->n = tp.own.n_steps = tp.own.n_threads = 0;
-      cluster_arrive();
+      if (ranks > 1) cluster_arrive();
     }
     // the warp that writes the row's numbers
     const bool writes = TOP ? rank == 0 && warp == kRowWarps - 1 : rank == turn_rank && warp == turn_warp;
@@ -989,28 +991,31 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
     if (S.edge >= 0) add_term<ENT>(t, xe, A.a);
     const float4 ws = warp_sums<ENT>(t, A.a);
     if constexpr (!TOP) {
-      if (lane == 0) join.warp[which][warp] = ws;
+      const int place = ranks == 1 ? turn_warp : which;
+      if (lane == 0) join.warp[place][warp] = ws;
       __syncwarp();
+      RowSums mine = {-INFINITY, 0.0, 0.0};
       if (warp == turn_warp) {
-        bar_sync(1 + which);
-        const RowSums mine = join_warps<ENT>(kRowWarps, A.a, [&](int i) { return join.warp[which][i]; });
-        if (waiting) cluster_wait();
+        bar_sync(1 + place);
+        mine = join_warps<ENT>(kRowWarps, A.a, [&](int i) { return join.warp[place][i]; });
         if (ranks == 1) write_row<T, ENT>(A, r, R, mine, y, xy);
-        else if (lane == 0) *cl.map_shared_rank(&join.cta[which][rank], turn_rank) = mine;
-        __syncwarp();
       } else {
-        bar_arrive(1 + which);
+        bar_arrive(1 + place);
+      }
+      if (ranks > 1) {
         if (waiting) cluster_wait();
+        if (warp == turn_warp && lane == 0) *cl.map_shared_rank(&join.cta[which][rank], turn_rank) = mine;
+        __syncwarp();
+        cluster_arrive();
+        waiting = true;
+        if (writes) {
+          cluster_wait();
+          waiting = false;
+          const RowSums sum = lane_sums<ENT>(lane < ranks ? join.cta[which][lane] : RowSums{-INFINITY, 0.0, 0.0}, A.a);
+          write_row<T, ENT>(A, r, R, sum, y, xy);
+        }
+        which ^= 1;
       }
-      cluster_arrive();
-      waiting = true;
-      if (ranks > 1 && writes) {
-        cluster_wait();
-        waiting = false;
-        const RowSums sum = lane_sums<ENT>(lane < ranks ? join.cta[which][lane] : RowSums{-INFINITY, 0.0, 0.0}, A.a);
-        write_row<T, ENT>(A, r, R, sum, y, xy);
-      }
-      which ^= 1;
       if (++turn_rank == ranks) {
         turn_rank = 0;
         turn_warp = turn_warp + 1 == kRowWarps ? 0 : turn_warp + 1;
@@ -1018,7 +1023,7 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
     } else {
       top_maxima(t.m, told, tp.red);
       __syncthreads();
-      cluster_wait();  // rank 0 is at this row
+      if (ranks > 1) cluster_wait();  // rank 0 is at this row
       float bound;
       if (alone) {
         bound = tp.red[rounds - 1][0];
@@ -1040,10 +1045,14 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
       }
       if (lane < 3) cl.map_shared_rank(&tp, 0)->warps[rank * kRowWarps + warp][lane] = lane == 0 ? ws.x : lane == 1 ? ws.z : ws.w;
       top_gather(R, S, steps, xe, bound, tp.own, cl.map_shared_rank(top, 0));
-      __syncwarp();
-      cluster_arrive();
-      cluster_wait();  // the gathered keys are rank 0's
-      if (rank != 0) continue;
+      if (ranks > 1) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+      } else {
+        __syncthreads();
+      }
+      if (rank != 0) continue;  // the gathered keys are rank 0's
       if (writes) {
         const RowSums sum = join_warps<ENT>(ranks * kRowWarps, A.a, [&](int i) {
           const float m = tp.warps[i][0];
@@ -1085,9 +1094,11 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
   }
   copies_wait<0>();
   if (waiting) cluster_wait();
-  __syncwarp();
-  cluster_arrive();  // no CTA ends while a peer may write to it or read from it
-  cluster_wait();
+  if (ranks > 1) {  // no CTA ends while a peer may write to it or read from it
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
 }
 
 // ---------------------------------------------------------------- backward
@@ -1388,17 +1399,28 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
     __syncthreads();
 
     // ---- the row's sums
-    if (warp == 0) {
-      const RowSums o = join_warps<false>(kRowWarps, A.a, [&](int i) { return J.warp[i]; });
-      const RowSums l = join_warps<false>(kRowWarps, A.a, [&](int i) { return J.warp_listed[i]; });
-      if (lane == 0) {
-        J.others = o;
-        J.listed = l;
+    auto others = [&](int i) { return J.warp[i]; };
+    auto of_list = [&](int i) { return J.warp_listed[i]; };
+    RowSums O, l;
+    // a CTA by itself: every warp joins the sums (without the gradient the third
+    // CTA an SM leaves no registers for that: 1024 x 151936 111 us against 102)
+    const bool each = GRAD && ranks == 1;
+    if (each) {
+      O = join_warps<false>(kRowWarps, A.a, others);
+      l = join_warps<false>(kRowWarps, A.a, of_list);
+    } else {
+      if (warp == 0) {
+        const RowSums o = join_warps<false>(kRowWarps, A.a, others);
+        const RowSums p = join_warps<false>(kRowWarps, A.a, of_list);
+        if (lane == 0) {
+          J.others = o;
+          J.listed = p;
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      if (ranks > 1) cluster_arrive();
     }
-    cluster_arrive();
-    prepare(list[which ^ 1], r + 2 * stride);  // meanwhile
+    prepare(list[which ^ 1], r + 2 * stride);  // in a cluster, meanwhile
     double Q = 0.0, log_top = 0.0;  // the teacher's mass; for logits, its log relative to the largest
     float top = 0.f;
     bool live = true;               // some entry is present
@@ -1424,15 +1446,18 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
     // an entry's log mass, and its mass
     auto log_q = [&] { return logits ? ((double)val - (double)top) * A.rT - log_top : (double)val; };
     auto mass = [&] { return id < 0 ? 0.0 : logits ? exp(log_q()) : L.q[tid]; };
-    cluster_wait();
-    RowSums O = {-INFINITY, 0.0, 0.0}, l = O;
-    if (lane < ranks) {
-      const DistillJoin* p = cl.map_shared_rank(&J, lane);
-      O = p->others;
-      l = p->listed;
+    if (!each) {
+      if (ranks > 1) cluster_wait();
+      else __syncthreads();
+      O = l = {-INFINITY, 0.0, 0.0};
+      if (lane < ranks) {
+        const DistillJoin* p = cl.map_shared_rank(&J, lane);
+        O = p->others;
+        l = p->listed;
+      }
+      O = lane_sums<false>(O, A.a);
+      l = lane_sums<false>(l, A.a);
     }
-    O = lane_sums<false>(O, A.a);
-    l = lane_sums<false>(l, A.a);
     const float m = fmaxf(O.m, l.m);
     // from the other ids' and the listed ones' maximum to the row's
     const double scale = O.m == -INFINITY ? 1.0 : (double)ex2_approx(below(O.m, m) * A.a);
@@ -1448,8 +1473,11 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
         loss = warp_sum(loss);
       }
       if (lane == 0) L.loss[warp] = loss;
-      __syncthreads();
-      if (tid == 0) {
+      __syncwarp();
+      if (warp < kRowWarps - 1) {  // the others are at the gradient while the last one adds up
+        bar_arrive(1);
+      } else {
+        bar_sync(1);
         loss = 0.0;
         for (int i = 0; i < kRowWarps; i++) loss += L.loss[i];
         if (rest != 0.0) {
@@ -1457,7 +1485,7 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
           loss += rest * (log(rest) - (log(O.s) + gap - log_s));
         }
         if (empty) loss = INFINITY;
-        A.loss[r] = live ? (float)loss : 0.f;
+        if (lane == 0) A.loss[r] = live ? (float)loss : 0.f;
       }
     }
 
@@ -1538,9 +1566,11 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
     }
   }
   copies_wait<0>();
-  __syncwarp();
-  cluster_arrive();  // no CTA ends while a peer may read from it
-  cluster_wait();
+  if (ranks > 1) {  // no CTA ends while a peer may read from it
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
 }
 
 template <typename F>
