@@ -1207,9 +1207,21 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
 // What is joined of a row: the sums of the ids not listed and of the listed
 // ones, the warps' and the CTA's (which the others of the cluster read).
 struct DistillJoin {
-  float4 warp[kRowWarps], warp_listed[kRowWarps];
+  float4 warp[kRowWarps];
+  RowSums warp_listed[kRowWarps];
   RowSums others, listed;
 };
+
+// exp((x - m) / T) in fp64, m being a maximum that x is part of.
+__device__ __forceinline__ double exact_term(float x, float m, double rT) {
+  return x == -INFINITY ? 0.0 : exp(((double)x - (m == -INFINITY ? 0.0 : (double)m)) * rT);
+}
+// lane_sums for the listed ids' masses, whose terms are few and exact.
+__device__ __forceinline__ RowSums lane_list(const RowSums& p, double rT) {
+  RowSums r = {warp_max_f(p.m), 0.0, 0.0};
+  r.s = warp_sum(p.m == -INFINITY ? p.s : p.s * exact_term(p.m, r.m, rT));
+  return r;
+}
 // The teacher's list of a row, and what its warps add up of it: the masses,
 // relative to exp(m / T) for a list of logits, and the terms of the loss.
 struct DistillList {
@@ -1379,7 +1391,7 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
       if (!listed) add_term<false>(t, xe, A.a);
     }
     const float4 ws = warp_sums<false>(t, A.a);
-    float4 wl = {-INFINITY, 0.f, 0.f, 0.f};
+    RowSums wl = {-INFINITY, 0.0, 0.0};
     bool first = inside, twice = false;  // an id's first place in the list stands for it
     if (warp * 32 < K) {
       if (inside)
@@ -1388,9 +1400,9 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
             twice = true;
             first &= tid < j;
           }
-      Sums tl;
-      if (first) add_term<false>(tl, xl, A.a);
-      wl = warp_sums<false>(tl, A.a);
+      // in fp64: p - q of a listed id is what is left of two close numbers
+      wl.m = warp_max_f(first ? xl : -INFINITY);  // a NaN is in no maximum, and in the sum
+      wl.s = warp_sum(first ? exact_term(xl, wl.m, A.rT) : 0.0);
     }
     if (lane == 0) {
       J.warp[warp] = ws;
@@ -1400,18 +1412,20 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
 
     // ---- the row's sums
     auto others = [&](int i) { return J.warp[i]; };
-    auto of_list = [&](int i) { return J.warp_listed[i]; };
+    auto listed = [&] {
+      return lane_list(lane < kRowWarps ? J.warp_listed[lane] : RowSums{-INFINITY, 0.0, 0.0}, A.rT);
+    };
     RowSums O, l;
     // a CTA by itself: every warp joins the sums (without the gradient the third
     // CTA an SM leaves no registers for that: 1024 x 151936 111 us against 102)
     const bool each = GRAD && ranks == 1;
     if (each) {
       O = join_warps<false>(kRowWarps, A.a, others);
-      l = join_warps<false>(kRowWarps, A.a, of_list);
+      l = listed();
     } else {
       if (warp == 0) {
         const RowSums o = join_warps<false>(kRowWarps, A.a, others);
-        const RowSums p = join_warps<false>(kRowWarps, A.a, of_list);
+        const RowSums p = listed();
         if (lane == 0) {
           J.others = o;
           J.listed = p;
@@ -1456,12 +1470,12 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
         l = p->listed;
       }
       O = lane_sums<false>(O, A.a);
-      l = lane_sums<false>(l, A.a);
+      l = lane_list(l, A.rT);
     }
     const float m = fmaxf(O.m, l.m);
     // from the other ids' and the listed ones' maximum to the row's
-    const double scale = O.m == -INFINITY ? 1.0 : (double)ex2_approx(below(O.m, m) * A.a);
-    const double scale_l = l.m == -INFINITY ? 1.0 : (double)ex2_approx(below(l.m, m) * A.a);
+    const double scale = O.m == -INFINITY ? 1.0 : exact_term(O.m, m, A.rT);
+    const double scale_l = l.m == -INFINITY ? 1.0 : exact_term(l.m, m, A.rT);
     const double s = O.s * scale + l.s * scale_l;
     const bool empty = s == 0.0;
     if (A.loss && mine) {
@@ -1560,8 +1574,7 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
             if (L.id[j] == id)
               qs += logits ? L.q[j] * exp(((double)L.m[j >> 5] - (double)top) * A.rT - log_top) : L.q[j];
         }
-        const double p = xl == -INFINITY ? 0.0 : (double)ex2_approx(below(xl, m) * A.a) / s;
-        d[id] = from_f<T>((float)(wt * (all * p - qs)));
+        d[id] = from_f<T>((float)(wt * (all * (exact_term(xl, m, A.rT) / s) - qs)));
       }
     }
   }

@@ -3,13 +3,14 @@ the kernels' arithmetic has to keep.
 
 Bounds, with u = 2^-24 (half a step of fp32, relative).  A term
 2^((x - m) a) with a = fp32(log2(e) / T) is off by
-  - the subtraction, the product and the rounding of a: 3 u |x - m| / T in the
-    exponent (nats),
+  - at most a subtraction or a reference's rounding, a product, and the rounding
+    of a: 3 u |x - m| / T in the exponent (nats),
   - the exponential: ex2.approx, 2^-22 relative = 4 u,
 and a thread adds at most `n` such terms in fp32 (n u relative, all terms being
-positive), with one rescaling (a term of its own, and a product) each time its
-maximum moves: at most 6 u for each of at most 16 moves counted here as 96 u.
-Sums over threads are in fp64.
+positive; fewer where it adds steps), with one rescaling (a term of its own, and
+a product) each time its maximum moves: at most 6 u for each of at most 16 moves
+counted here as 96 u, in which a warp's five fp32 additions are too.  Sums over
+warps are in fp64.
 """
 import math
 
@@ -174,7 +175,7 @@ def distill(x, T, ids, values, kind, weight, dtype):
         log_R, tail = -np.inf, 0.0
     if rest > 0:
         loss += rest * (math.log(rest) - log_R)
-    eps_s = R.eps_s  # the listed ids' terms are fp32 terms like the others
+    eps_s = eps_t * tail  # the listed ids' terms are in fp64
     b_loss = 0.0
     if np.isfinite(loss):
         b_loss = (Q + rest) * eps_s + rest * eps_t + abs(loss) * U + 1e-12
@@ -182,8 +183,7 @@ def distill(x, T, ids, values, kind, weight, dtype):
         return loss, b_loss, zero, zero
     all_ = Q + rest
     dx = np.where(listed, R.p * all_ - mass, 0.0)
-    far = np.where(R.p > 0, -R.d, 0.0)
-    b = np.where(listed, R.p * all_ * (eps_s + (3 * far + 4) * U) + 1e-13, 0.0)
+    b = np.where(listed, R.p * all_ * eps_s + 1e-13, 0.0)
     if not tail_empty:
         share = np.zeros(V)
         share[~listed] = po
