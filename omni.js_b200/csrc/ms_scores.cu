@@ -41,7 +41,8 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 // 16-byte vectors of a thread's step.  2 instead, with twice the steps in flight
-// (same bytes): 2048 x 151936 bf16 103 -> 114 us, distillation of 4096 rows 537 -> 556 us.
+// (same bytes): 2048 x 151936 bf16 102 -> 115 us, 512 x 262144 top 64 130 -> 142,
+// distillation of 4096 x 151936 540 -> 551.
 constexpr int kBatch = 4;
 constexpr int kMaxCluster = 16;
 constexpr int kBuf = 992;       // keys the selection holds (runs of 32)
@@ -602,9 +603,9 @@ struct TopSmem {
 
 // Up to this many (CTAs a row) * (bounds) a CTA goes by its own bound; beyond,
 // the CTAs meet first to find the row's.  Meeting costs about 1 us of a row and
-// leaves fewer keys: one row of 50257, top 5, 7 CTAs (7): 9.9 us alone, 10.4 met;
-// 16 CTAs (16): 12.5 alone, 11.5 met; 64 x 128256 top 20, 4 CTAs (12): 20.0 alone,
-// 17.8 met; 512 x 262144 top 64, 2 CTAs (16): 199 alone, 176 met.
+// leaves fewer keys: one row of 50257, top 5, 7 CTAs (7): 10.0 us alone, 10.5 met;
+// 16 CTAs (16): 12.3 alone, 11.3 met; 64 x 128256 top 20, 4 CTAs (12): 18.4 alone,
+// 17.5 met; 512 x 262144 top 64, 2 CTAs (16): 130 alone, 128 met.
 constexpr int kAlone = 10;
 constexpr int kRounds = kScoreMax / kRowWarps;  // bounds that a CTA gives for the largest top_n
 
@@ -817,9 +818,10 @@ __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
 // ---------------------------------------------------------------- forward
 // CTAs an SM and steps of their rings: 96 KiB in flight an SM.  Every other load
 // (tokens, the alternatives' second read) waits behind what the rings have asked
-// for: with 4 steps 512 x 262144 top 64 takes 162 us instead of 139, and
-// 2048 x 151936 bf16 105 instead of 103.  4 CTAs, at 64 registers: 175 and 120 us;
-// 2 CTAs with 6 steps: 205 and 112 us.
+// for.  us of 2048 x 151936 bf16, 512 x 262144 top 64, 333 x 50257 top 3:
+// 102, 130, 16; with 3 steps 102, 128, 17; with 4 (and so 2 CTAs where there are
+// alternatives) 102, 120, 23; 4 CTAs, at 64 registers, 121, 130, 17; 2 CTAs with
+// 6 steps 112, 125, 21.
 constexpr int kScoreCtas = 3, kScoreDepth = 2;
 constexpr int kScoreRing = kScoreDepth * kBatch * kRowThreads * 16;
 
@@ -1241,9 +1243,9 @@ __device__ __forceinline__ void zero_slice(const Row<T>& R, const Slice<T>& S, T
 }
 
 // CTAs an SM, and steps of their rings.  The gradient's second loop takes the
-// registers of a third CTA: 4096 x 151936 bf16 with gradient 537 us, with three
-// CTAs that spill 567; the loss alone, 1024 x 151936 with 256 listed ids, 100 us
-// with three, 120 with two.  Of the rings' steps: 2 580 us, 3 538, 4 546, 6 542.
+// registers of a third CTA: 4096 x 151936 bf16 with gradient 540 us, with three
+// CTAs that spill 570; the loss alone, 1024 x 151936 with 256 listed ids, 104 us
+// with three, 123 with two.  With rings of 2 steps 571 us, of 4 and of 6 560.
 template <bool GRAD>
 struct DistillShape {
   static constexpr int kCtas = GRAD ? 2 : 3, kDepth = GRAD ? 3 : 2, kRing = kDepth * kBatch * kRowThreads * 16;
@@ -1658,7 +1660,10 @@ cudaError_t row_clusters(void (*kernel)(Args), int ring, const RowClusters** fou
 // the clusters in rounds, so the time is about rounds * (slice + what a row
 // costs its CTAs beside the copies), in bytes at a CTA's share of the
 // bandwidth: `one` for a CTA by itself, `joined` where CTAs meet, and 2 KiB for
-// each of them.
+// each of them.  The figures are fitted to timings of every size; what a wrong
+// choice costs, in us: 2048 x 151936 bf16 1 CTA 102, 2 121; one row of 50257 1 CTA
+// 12.8, 2 10.5, 6 9.5, 16 11.3; 512 x 262144 top 64 1 CTA 134, 3 126, 4 130, 7 167;
+// distillation of 1024 x 128256 1 CTA 132, 2 154, and of 8 x 262144 54, 31, 14 (16).
 int best_ranks(const RowClusters& k, int64_t B, int64_t row_bytes, int fit, int64_t one, int64_t joined) {
   int best = 0;
   int64_t least = INT64_MAX;
@@ -1698,7 +1703,7 @@ cudaError_t launch_logprobs(const ScoreArgs& A, int dtype, cudaStream_t stream) 
     const RowClusters* rc = nullptr;
     const cudaError_t e = row_clusters(k, kScoreRing, &rc);
     if (e != cudaSuccess) return e;
-    const int ranks = best_ranks(*rc, A.B, (int64_t)A.V * sizeof(T), fit, 16384, top ? 32768 : 24576);
+    const int ranks = best_ranks(*rc, A.B, (int64_t)A.V * sizeof(T), fit, 16384, top ? 98304 : 24576);
     return launch_rows(k, A, *rc, ranks, kScoreRing, stream);
   });
 }
