@@ -117,6 +117,66 @@ def test_top_alternatives(sampler, top_n, V):
         _check_score(sampler, x, 1.0, None, top_n)
 
 
+@pytest.mark.parametrize("B,V,dtype,top_n", [(512, 262144, "float32", 64), (512, 262144, "bfloat16", 200),
+                                             (1100, 65537, "float16", 0), (460, 131075, "float32", 3)])
+def test_rows_over_several_rounds(sampler, B, V, dtype, top_n):
+    """More rows than the GPU takes at once, padding among them, rows of one and of several CTAs: rows of
+    every round against the oracle, all of them against a call of their own few rows."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(B + top_n)
+    x = _placed((torch.randn(B, V, device="cuda", generator=g) * 2.5).to(_torch(dtype)), 1, 2)
+    tok = torch.randint(0, V, (B, 1), device="cuda", generator=g, dtype=torch.int32)
+    tok[::7] = -1
+    o = sampler.logprobs(x, tok, top_n=top_n, entropy=True, stats=True)
+    torch.cuda.synchronize()
+    for r in [0, 1, 7, 147, 148, 295, 296, 443, 444, B - 2, B - 1]:
+        if r >= B:
+            continue
+        want, bound = O.score(_np(x[r]), 1.0, tok[r].tolist(), top_n)
+        for k, v in want.items():
+            got = _np(getattr(o, k))
+            if got is not None:
+                _near(np.atleast_1d(got[r]), np.atleast_1d(v), bound[k], (k, r))
+    if top_n:
+        live = (tok >= 0).flatten()
+        xf = x.float()
+        got = torch.gather(xf, 1, o.top_ids.clamp(min=0).long())[live]
+        assert torch.equal(got, torch.topk(xf, top_n, dim=1).values[live])
+        assert bool((o.top_ids[~live] == -1).all())
+    few = [sampler.logprobs(x[r:r + 50], tok[r:r + 50], entropy=True) for r in range(0, B, 50)]
+    # both within the sums' bound of the truth, which is some hundred 2^-24 of a value near 10
+    assert torch.allclose(o.entropy, torch.cat([f.entropy for f in few]), rtol=2.0 ** -15, atol=0)
+    assert torch.allclose(o.logprobs, torch.cat([f.logprobs for f in few]), rtol=2.0 ** -15, atol=2.0 ** -15)
+
+
+@pytest.mark.parametrize("B,V,dtype,K", [(300, 262144, "float32", 40), (700, 50259, "bfloat16", 256)])
+def test_distill_rows_over_several_rounds(sampler, B, V, dtype, K):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = _placed((torch.randn(B, V, device="cuda", generator=g) * 2.5).to(_torch(dtype)), 1, 2)
+    v, ids = torch.topk(x.float() + 0.7 * torch.randn(B, V, device="cuda", generator=g), K, dim=1)
+    v, ids = torch.log_softmax(v, 1) - 0.05, ids.to(torch.int32)
+    ids[::5] = -1
+    w = torch.rand(B, device="cuda", generator=g)
+    w[3::11] = 0.0
+    loss, dx = sampler.distill_grad(x, ids, v, w)
+    assert torch.equal(loss, sampler.distill_loss(x, ids, v))
+    torch.cuda.synchronize()
+    for r in [0, 1, 3, 14, 147, 148, 295, 296, 297, B - 2, B - 1]:
+        if r >= B:
+            continue
+        wl, bl, wd, bd = O.distill(_np(x[r]), 1.0, ids[r].tolist(), _np(v[r]), "logprobs", float(w[r]), dtype)
+        _near([_np(loss)[r]], [wl], bl, ("loss", r))
+        _near(_np(dx[r]), wd, bd, ("dlogits", r))
+    # the gradient of a row of weight sums to 0, the softmax's, up to its elements' rounding
+    live = (ids >= 0).any(1) & (w != 0)
+    assert bool((dx[~live] == 0).all())
+    big = dx.double().abs().sum(1)
+    assert bool((dx.double().sum(1).abs()[live] <= big[live] * (2.0 ** -8 if dtype == "bfloat16" else 2.0 ** -18)).all())
+
+
 def _shaped(kind, V, rng):
     i = np.arange(V)
     if kind == "constant":
