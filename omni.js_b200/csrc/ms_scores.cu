@@ -45,7 +45,7 @@ constexpr int kRowWarps = kRowThreads / 32;
 // distillation of 4096 x 151936 540 -> 551.
 constexpr int kBatch = 4;
 constexpr int kMaxCluster = 16;
-constexpr int kBuf = 992;       // keys the selection holds (runs of 32)
+constexpr int kBuf = 2048;      // keys the selection holds (runs of 32)
 constexpr int kScan = 512;      // of them, those that the tiled selection uses: top_n and a tile of kRowThreads
 
 // ---------------------------------------------------------------- row access
@@ -925,7 +925,6 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
   const int share = min(rounds, (2 * rounds + ranks - 1) / ranks + 2);
   // with few CTAs or alternatives each CTA's own bound leaves few enough elements
   const bool alone = ranks == 1 || ranks * rounds <= kAlone;
-  const int told = alone ? rounds : share;
   const int64_t first = blockIdx.x / ranks, step = gridDim.x / ranks;
   const ms_scores& O = A.out;
   Feed<T, kScoreDepth> feed;
@@ -1023,14 +1022,20 @@ __global__ void __launch_bounds__(kRowThreads, kScoreCtas) logprobs_kernel(Score
         turn_warp = turn_warp + 1 == kRowWarps ? 0 : turn_warp + 1;
       }
     } else {
+      // Its own bound: from the warps all of whose threads hold vectors (in a
+      // short slice not all do), each with its share of top_n; none where a
+      // warp's 32 threads are too few for that.
+      const int full = min(kRowWarps, (S.w1 - S.w0) / 32), own = full > 0 ? (A.top_n + full - 1) / full : 33;
+      const int told = alone ? (own <= 32 ? own : 0) : share;
       top_maxima(t.m, told, tp.red);
       __syncthreads();
       if (ranks > 1) cluster_wait();  // rank 0 is at this row
-      float bound;
+      float bound = -INFINITY;
       if (alone) {
-        bound = tp.red[rounds - 1][0];
-#pragma unroll
-        for (int w = 1; w < kRowWarps; w++) bound = fminf(bound, tp.red[rounds - 1][w]);
+        if (told > 0) {
+          bound = INFINITY;
+          for (int w = 0; w < full; w++) bound = fminf(bound, tp.red[told - 1][w]);
+        }
       } else {
         if (tid < told) {
           float b = tp.red[tid][0];

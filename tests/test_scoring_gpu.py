@@ -106,7 +106,7 @@ def test_score_temperatures(sampler, T):
 
 
 @pytest.mark.parametrize("top_n", [1, 2, 31, 32, 33, 64, 100, 255, 256])
-@pytest.mark.parametrize("V", [7, 300, 5000, 40000])
+@pytest.mark.parametrize("V", [7, 300, 1030, 1500, 2049, 5000, 40000])
 def test_top_alternatives(sampler, top_n, V):
     """Continuous values, and a few distinct values only (ties by ascending id)."""
     rng = np.random.default_rng(top_n)
