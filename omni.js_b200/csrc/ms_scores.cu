@@ -721,17 +721,20 @@ struct TopOwners {
 // steps whose maximum reaches the bound hold any; a thread knows its two
 // largest, and only where a third reaches the bound too are all of its steps
 // read.  All threads read those vectors together, out of L2 or HBM (every step
-// of those threads instead: 512 x 262144 top 64 142 us, against 129).  Keys
-// beyond the buffer are counted and left out.  xe: the thread's edge element.
+// of those threads instead: 512 x 262144 top 64 142 us, against 129).  A
+// thread that finds the buffer full leaves the count above kBuf and takes no
+// more keys.  xe: the thread's edge element.
 template <typename T>
 __device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, const TopSteps& t, float xe, float bound,
                                            TopOwners& own, TopSmem* to) {
   constexpr int VEC = Row<T>::VEC, AHEAD = 4;
   const uint4* base = reinterpret_cast<const uint4*>(R.p - R.mis);
+  bool room = true;  // as far as this thread has seen
   auto take = [&](float x, int i) {
-    if (x >= bound && x > -INFINITY) {
+    if (room && x >= bound && x > -INFINITY) {
       const int n = atomicAdd(&to->n, 1);
-      if (n < kBuf) to->key[n] = top_key(x, i);
+      room = n < kBuf;
+      if (room) to->key[n] = top_key(x, i);
     }
   };
   auto take_vec = [&](int v, const uint4& u) {
@@ -751,14 +754,14 @@ __device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, c
   if (S.edge >= 0) take(xe, S.edge);
   __syncthreads();
 #pragma unroll 1
-  for (int i = threadIdx.x; i < own.n_steps * kBatch; i += kRowThreads) {
+  for (int i = threadIdx.x; room && i < own.n_steps * kBatch; i += kRowThreads) {
     const uint32_t o = own.step[i / kBatch];
     const int v = S.w0 + (int)(o & 0xffu) + ((int)(o >> 8) * kBatch + i % kBatch) * kRowThreads;
     if (v < S.w1) take_vec(v, base[v]);
   }
   const int n = own.n_threads, each = (S.w1 - S.w0 + kRowThreads - 1) / kRowThreads;
 #pragma unroll 1
-  for (int i = threadIdx.x; i < n * each; i += AHEAD * kRowThreads) {
+  for (int i = threadIdx.x; room && i < n * each; i += AHEAD * kRowThreads) {
     uint4 u[AHEAD];
     int v[AHEAD];
 #pragma unroll
@@ -777,41 +780,68 @@ __device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, c
 // row's finite elements).  One element a thread at a time goes in when it
 // beats the n-th best of those sorted so far; the buffer is sorted and cut
 // back to top_n whenever the next tile might not fit.  Right for every row.
+// Tiles come in order of their ids, so an element that only equals the n-th
+// best of earlier tiles loses to it: tiles without a larger one are passed
+// over, which is most of a row that ties by the thousand (10 finite logits
+// among the type's lowest value, top 20, 64 x 128256 fp32: 74 us; each
+// tile element by element 156).
 template <typename T>
 __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
-  constexpr int VEC = Row<T>::VEC;
+  constexpr int VEC = Row<T>::VEC, AHEAD = 4;
   unsigned long long thr = 0;
+  float least = -INFINITY;  // thr's logit
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  const int tiles = (R.nvec + (int)blockDim.x - 1) / (int)blockDim.x;
-  for (int t = 0; t < tiles; t++) {
-    const int v = t * blockDim.x + threadIdx.x;
-    float f[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; j++) f[j] = -INFINITY;
-    if (v < R.nvec) load_vec(R, v, f);
+  const int tiles = (R.nvec + kRowThreads - 1) / kRowThreads;
 #pragma unroll 1
-    for (int j = 0; j < VEC; j++) {
-      float x = f[0];
+  for (int t0 = 0; t0 < tiles; t0 += AHEAD) {
+    float hi[AHEAD];
 #pragma unroll
-      for (int l = 1; l < VEC; l++) x = l == j ? f[l] : x;
-      const unsigned long long k = x > -INFINITY ? top_key(x, v * VEC - R.mis + j) : 0ull;
-      if (k > thr) sh.key[atomicAdd(&sh.n, 1)] = k;
-      __syncthreads();
-      const int n = sh.n;
-      __syncthreads();
-      if (n + (int)blockDim.x > kScan) {
-        for (int i = n + threadIdx.x; i < kScan; i += blockDim.x) sh.key[i] = 0;
-        sort_desc(sh.key, kScan);
-        thr = sh.key[top_n - 1];
+    for (int a = 0; a < AHEAD; a++) {
+      const int v = (t0 + a) * kRowThreads + threadIdx.x;
+      hi[a] = -INFINITY;
+      if (v >= R.nvec) continue;
+      float f[VEC];
+      load_vec(R, v, f);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) hi[a] = fmaxf(hi[a], f[j]);
+    }
+    float any = hi[0];
+#pragma unroll
+    for (int a = 1; a < AHEAD; a++) any = fmaxf(any, hi[a]);
+    if (!__syncthreads_or(any > least)) continue;
+#pragma unroll
+    for (int a = 0; a < AHEAD; a++) {
+      if (!__syncthreads_or(hi[a] > least)) continue;
+      const int v = (t0 + a) * kRowThreads + threadIdx.x;
+      float f[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j++) f[j] = -INFINITY;
+      if (v < R.nvec) load_vec(R, v, f);
+#pragma unroll 1
+      for (int j = 0; j < VEC; j++) {
+        float x = f[0];
+#pragma unroll
+        for (int l = 1; l < VEC; l++) x = l == j ? f[l] : x;
+        const unsigned long long k = x > -INFINITY ? top_key(x, v * VEC - R.mis + j) : 0ull;
+        if (k > thr) sh.key[atomicAdd(&sh.n, 1)] = k;
         __syncthreads();
-        if (threadIdx.x == 0) sh.n = top_n;
+        const int n = sh.n;
         __syncthreads();
+        if (n + kRowThreads > kScan) {
+          for (int i = n + threadIdx.x; i < kScan; i += kRowThreads) sh.key[i] = 0;
+          sort_desc(sh.key, kScan);
+          thr = sh.key[top_n - 1];
+          least = fkey_inv((uint32_t)(thr >> 32));
+          __syncthreads();
+          if (threadIdx.x == 0) sh.n = top_n;
+          __syncthreads();
+        }
       }
     }
   }
   const int n = sh.n;
-  for (int i = n + threadIdx.x; i < kScan; i += blockDim.x) sh.key[i] = 0;
+  for (int i = n + threadIdx.x; i < kScan; i += kRowThreads) sh.key[i] = 0;
   sort_desc(sh.key, kScan);
 }
 
