@@ -175,7 +175,7 @@ def logprobs_backward(s, logits, tokens, row_max, row_sum, g_logprobs=None, g_en
         entropy = _rows(entropy, "entropy", logits, torch.float32, (B,))
     dx = _grad_out(s, logits, out)
     s._check(s._L.ms_logprobs_backward(s._ctx, logits.data_ptr(), dtype, B, V, ld, float(temperature), _p(tok),
-                                       n,                                        row_max.data_ptr(), row_sum.data_ptr(), _p(entropy), _p(g_logprobs),
+                                       n, row_max.data_ptr(), row_sum.data_ptr(), _p(entropy), _p(g_logprobs),
                                        _p(g_entropy), dx.data_ptr(), dx.stride(0), _current(s)))
     return dx
 
