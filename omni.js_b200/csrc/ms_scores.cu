@@ -153,15 +153,19 @@ __device__ __forceinline__ void store_vec(const Row<T>& R, T* d, bool same, int 
 // Sums over some of a thread's elements: their maximum m (-Inf while there is
 // none), z = fp32(m a), and with y = x a - z, one rounding each,
 // s = sum 2^y and q = sum 2^y y, in two halves (the lanes of the paired fp32
-// instructions).  What z's rounding leaves, z - m a, is put right in fp64 when
-// the threads' sums are joined.  Where m a is beyond fp32 (|m| > 2e38: a row of
-// nothing but a type's lowest value, an Inf), y = (x - m) a instead.
+// instructions).  What z's rounding leaves, z - m a, is in every term, and is put
+// right in fp64 when the threads' sums are joined.  It is at most 2^-25 |z|: half
+// a unit below kFar, but beyond fp32's exponents for a mask of -1e10 or a type's
+// lowest value.  Where z is that large (or an Inf) the reference is m a itself,
+// y = (x - m) a, an instruction more an element.
 typedef unsigned long long f32x2;
 struct Sums {
   float m = -INFINITY, z = 0.f;
   f32x2 s = 0, q = 0;
-  bool odd = false;  // masked elements (0 times their y of -Inf), or m a beyond fp32: each term with care from here on
+  bool odd = false;  // masked elements (0 times their y of -Inf): each term with care from here on
 };
+constexpr float kFar = 16777216.f;  // 2^24
+__device__ __forceinline__ bool far(float z) { return !(fabsf(z) < kFar); }
 
 // y, bounded below so that a term of 0 times it is 0 (a NaN stays one)
 __device__ __forceinline__ float bounded(float d) {
@@ -184,7 +188,11 @@ __device__ __forceinline__ float warp_max_f(float v) {
 // The step from a reference (m, z) to (M, Z), M >= m, in units of y.
 __device__ __forceinline__ float step_of(float m, float z, float M, float Z, float a) {
   if (m == -INFINITY) return 0.f;  // sums of nothing (0), or of NaN alone: both stay
-  return bounded(isinf(Z) || isinf(z) ? __fsub_rn(m, M) * a : __fsub_rn(z, Z));
+  if (!far(z) && !far(Z)) return bounded(__fsub_rn(z, Z));
+  float d = __fsub_rn(m, M) * a;
+  if (!far(z)) d += fmaf(-m, a, z);
+  if (!far(Z)) d += fmaf(M, a, -Z);
+  return bounded(d);
 }
 
 // A word of a vector as two fp32 elements (of 4-byte types: two words).
@@ -240,7 +248,7 @@ __device__ __forceinline__ float add_words(Sums& t, const uint32_t (&w)[N], floa
   if (hi > t.m) raise_to<ENT>(t, hi, a);
   // The words' own sum first, then onto the thread's: its roundings grow with
   // the thread's steps and not with its elements.
-  if (!t.odd) {
+  if (!t.odd && !far(t.z)) {
     const f32x2 z2 = f2_pack(-t.z, -t.z), a2 = f2_pack(a, a);
     f32x2 s = 0, q = 0;
 #pragma unroll
@@ -251,10 +259,9 @@ __device__ __forceinline__ float add_words(Sums& t, const uint32_t (&w)[N], floa
       s = i == 0 ? e : f2_add(s, e);
       if constexpr (ENT) q = i == 0 ? f2_mul(e, y2) : f2_fma(e, y2, q);
     }
-    t.odd = isinf(t.z);
     if constexpr (ENT) {
       const float2 h = f2_unpack(q);
-      t.odd |= isnan(h.x + h.y);
+      t.odd = isnan(h.x + h.y);
     }
     if (!t.odd) {
       t.s = f2_add(t.s, s);
@@ -263,12 +270,13 @@ __device__ __forceinline__ float add_words(Sums& t, const uint32_t (&w)[N], floa
     }
   }
   const float m = t.m == -INFINITY ? 0.f : t.m;
+  const bool from_m = far(t.z);
   f32x2 s = 0, q = 0;
 #pragma unroll
   for (int i = 0; i < N; i += PER) {
     const float2 x = f2_unpack(pair_of(w[i], w[i + PER - 1], T()));
-    const float y0 = bounded(isinf(t.z) ? __fsub_rn(x.x, m) * a : fmaf(x.x, a, -t.z));
-    const float y1 = bounded(isinf(t.z) ? __fsub_rn(x.y, m) * a : fmaf(x.y, a, -t.z));
+    const float y0 = bounded(from_m ? __fsub_rn(x.x, m) * a : fmaf(x.x, a, -t.z));
+    const float y1 = bounded(from_m ? __fsub_rn(x.y, m) * a : fmaf(x.y, a, -t.z));
     const f32x2 e = f2_pack(ex2_approx(y0), ex2_approx(y1));
     s = i == 0 ? e : f2_add(s, e);
     if constexpr (ENT) q = i == 0 ? f2_mul(e, f2_pack(y0, y1)) : f2_fma(e, f2_pack(y0, y1), q);
@@ -317,7 +325,7 @@ __device__ __forceinline__ double exp_small(double d) {
 __device__ __forceinline__ RowSums exact_sums(float4 w, float a) {
   const double ln2 = 0.693147180559945309417;
   RowSums r = {w.x, (double)w.z, (double)w.w * ln2};
-  if (w.x != -INFINITY && !isinf(w.y)) {
+  if (w.x != -INFINITY && !far(w.y)) {
     const double d = ((double)w.y - (double)w.x * (double)a) * ln2;  // |d| <= |z| 2^-24
     const double c = exp_small(d);
     r.q = (r.q + r.s * d) * c;
@@ -1548,10 +1556,10 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
     // listed ids is overwritten below.
     const float mo = O.m == -INFINITY ? 0.f : O.m, zo = mo * A.a;
     double cd = O.s == 0.0 ? 0.0 : wt * (all * (scale / s) - rest / O.s);
-    if (!isinf(zo)) cd *= exp_small(((double)zo - (double)mo * (double)A.a) * 0.693147180559945309417);
+    if (!far(zo)) cd *= exp_small(((double)zo - (double)mo * (double)A.a) * 0.693147180559945309417);
     const float c = (float)cd;
-    auto term = [&](float x) { return c * ex2_approx(isinf(zo) ? __fsub_rn(x, mo) * A.a : fmaf(x, A.a, -zo)); };
-    const bool plain = same && !isinf(zo);
+    auto term = [&](float x) { return c * ex2_approx(far(zo) ? __fsub_rn(x, mo) * A.a : fmaf(x, A.a, -zo)); };
+    const bool plain = same && !far(zo);
     const f32x2 a2 = f2_pack(A.a, A.a), z2 = f2_pack(-zo, -zo), c2 = f2_pack(c, c);
     // n of the step's vectors, the first being the row's v
     auto put = [&](int v, uint32_t at, int n) {

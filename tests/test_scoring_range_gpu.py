@@ -1,0 +1,88 @@
+"""Scoring operators over the whole range of finite logits and of temperatures, against the 64-bit oracle within
+the bounds that it derives."""
+import numpy as np
+import pytest
+
+from test_scoring_gpu import _block, _check_distill, _check_grad, _check_score, _np, _torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["float32", "bfloat16", "float16"]
+# masks that callers write instead of -Inf, and large logits
+LARGE = [-1e9, -1e10, -1e20, -1e30, "lowest", 1e10, 1e30]
+LOWEST = {"float32": 3.4028234663852886e38, "bfloat16": 3.3895313892515355e38, "float16": 65504.0}  # but for the sign
+LARGE_OF = [(d, v) for d in DTYPES for v in LARGE if v == "lowest" or abs(v) <= LOWEST[d]]
+
+
+def _large(dtype, value):
+    """The value as the type holds it."""
+    import torch
+
+    return -LOWEST[dtype] if value == "lowest" else torch.tensor(value).to(_torch(dtype)).item()
+
+
+def _large_rows(dtype, value, V, seed=5):
+    """All of one value; all but the last tenth, but the first tenth, but every second id, but one id."""
+    x = _block(np.random.default_rng(seed), 5, V, dtype, 1, 3)
+    x[0] = value
+    x[1, : V - V // 10] = value
+    x[2, V // 10:] = value
+    x[3, ::2] = value
+    x[4, : V // 2] = value
+    x[4, V // 2 + 1:] = value
+    return x
+
+
+@pytest.mark.parametrize("T,dtype,value", [(T, d, v) for T in (0.001, 0.5, 1.0, 1.5, 2.0, 4.0, 10.0, 10000.0)
+                                           for d, v in LARGE_OF
+                                           if abs(LOWEST[d] if v == "lowest" else v) / T <= LOWEST["float32"]])
+def test_score_of_large_logits(sampler, T, dtype, value):
+    """Rows and parts of rows of one large value, in long rows too, where a thread has several steps of it; where
+    the log-probability of a mask is an fp32 number."""
+    v = _large(dtype, value)
+    for V in (5003, 150011):
+        x = _large_rows(dtype, v, V)
+        o = _check_score(sampler, x, T, [[0, V // 2, V - 1]] * 5, 5)
+        assert np.isfinite(_np(o.entropy)).all()
+
+
+@pytest.mark.parametrize("T", [0.25, 1.0, 3.0])
+@pytest.mark.parametrize("middle", [2.0 ** 23, 2.0 ** 24, 2.0 ** 25, 2.0 ** 30])
+def test_score_of_close_large_logits(sampler, T, middle):
+    """Logits some steps of fp32 around a number whose reference in the exponents' unit is near 2^24, below or above."""
+    import torch
+
+    rng = np.random.default_rng(int(middle))
+    c = np.float32(middle * T / 1.4426950408889634)
+    for sign in (-1, 1):
+        n = rng.integers(-12, 13, (4, 30011))
+        x = torch.from_numpy((sign * c * (1 + n * 2.0 ** -23)).astype(np.float32)).cuda()
+        _check_score(sampler, x, T, [[1, 30010]] * 4, 9)
+        _check_grad(sampler, x, T, [[1, 30010]] * 4, [[0.5, -0.25]] * 4, None)
+
+
+@pytest.mark.parametrize("dtype,value", LARGE_OF)
+def test_score_gradient_of_large_logits(sampler, dtype, value):
+    v = _large(dtype, value)
+    V = 5003
+    x = _large_rows(dtype, v, V)
+    for T in (0.7, 2.0, 10.0):
+        _check_grad(sampler, x, T, [[0, V // 2, V - 1]] * 5, [[0.5, -1.0, 0.25]] * 5, None)
+
+
+@pytest.mark.parametrize("dtype,value", LARGE_OF)
+@pytest.mark.parametrize("kind", ["logits", "logprobs"])
+def test_distill_of_large_logits(sampler, dtype, value, kind):
+    """One large value everywhere, in most of a row, at listed ids, and at every id that is not listed."""
+    import torch
+
+    v = _large(dtype, value)
+    for V in (2003, 150011):
+        x = torch.cat([_large_rows(dtype, v, V), _block(np.random.default_rng(6), 2, V, dtype)])
+        ids = [[5, 9, V // 2, V - 1]] * 7
+        x[5] = v
+        x[5, ids[5]] = torch.tensor([1.0, 2.0, 0.5, -1.0], dtype=x.dtype, device="cuda")
+        x[6, [9, V - 1]] = v
+        q = np.log(np.array([[0.4, 0.3, 0.2, 0.05]] * 7))
+        for T in (1.0, 1.5, 2.0, 4.0, 10.0):
+            _check_distill(sampler, x, T, ids, q.tolist(), kind, [1.0, 0.5, 1.0, 2.0, 1.0, 1.0, 0.25])
