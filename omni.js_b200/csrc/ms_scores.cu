@@ -167,12 +167,14 @@ struct Sums {
 constexpr float kFar = 16777216.f;  // 2^24
 __device__ __forceinline__ bool far(float z) { return !(fabsf(z) < kFar); }
 
-// y, bounded below so that a term of 0 times it is 0 (a NaN stays one)
-__device__ __forceinline__ float bounded(float d) {
+// the larger of two, NaN when one of them is
+__device__ __forceinline__ float max_or_nan(float a, float b) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d), "f"(-1e30f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// y, bounded below so that a term of 0 times it is 0 (a NaN stays one)
+__device__ __forceinline__ float bounded(float d) { return max_or_nan(d, -1e30f); }
 __device__ __forceinline__ float below(float x, float m) { return bounded(__fsub_rn(x, m)); }
 __device__ __forceinline__ f32x2 f2_mul(f32x2 a, f32x2 b) {
   f32x2 d;
@@ -1205,12 +1207,16 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
   const double k = -A.rT / S;
   const float c0 = (float)(k * (G + gH * (H - log_s)));
   const float c1 = (float)(k * gH * A.rT);
+  // e (c0 + c1 (x - m)), x - m bounded below where e is 0 already: masks lie so far
+  // off that c1 times their distance is beyond fp32 (T 0.001, g_H 655), and 0 times that NaN
+  const float lowest = -256.f / A.a;
+  auto term = [&](float x) {
+    const float dd = max_or_nan(__fsub_rn(x, m), lowest);
+    return ex2_approx(dd * A.a) * fmaf(c1, dd, c0);
+  };
   auto put = [&](int v, float(&f)[VEC]) {
 #pragma unroll
-    for (int j = 0; j < VEC; j++) {
-      const float dd = below(f[j], m);
-      f[j] = ex2_approx(dd * A.a) * fmaf(c1, dd, c0);
-    }
+    for (int j = 0; j < VEC; j++) f[j] = term(f[j]);
     store_vec(R, d, same, v, f);
   };
   if (zero) {
@@ -1243,8 +1249,7 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
         g += (double)s_g[u];
       }
     if (!first) continue;  // the same token twice: its first place writes the sum
-    const float dd = below(s_x[t], m);
-    d[y] = from_f<T>((float)(g * A.rT + (double)(ex2_approx(dd * A.a) * fmaf(c1, dd, c0))));
+    d[y] = from_f<T>((float)(g * A.rT + (double)term(s_x[t])));
   }
 }
 

@@ -86,3 +86,27 @@ def test_distill_of_large_logits(sampler, dtype, value, kind):
         q = np.log(np.array([[0.4, 0.3, 0.2, 0.05]] * 7))
         for T in (1.0, 1.5, 2.0, 4.0, 10.0):
             _check_distill(sampler, x, T, ids, q.tolist(), kind, [1.0, 0.5, 1.0, 2.0, 1.0, 1.0, 0.25])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [0.00011, 0.001, 0.01, 0.1, 1.0, 30.0, 10000.0])
+def test_score_gradient_of_masked_rows_at_any_temperature(sampler, dtype, T):
+    """Masks of -Inf and of the type's lowest value, masked tokens, entropy gradients as a loss scale leaves them.
+    fp16: such that the gradient of an id that is not masked stays finite."""
+    import torch
+
+    V = 2051
+    low = torch.finfo(_torch(dtype)).min
+    x = _block(np.random.default_rng(8), 6, V, dtype, 1, 1)
+    x[0, ::2] = -float("inf")
+    x[1, ::2] = low
+    x[2, : V - 3] = -float("inf")
+    x[3, 3:] = low
+    x[4] = -float("inf")
+    x[4, 77] = 2.0
+    tokens = [[0, 1], [2, 2000], [5, V - 1], [1, 100], [77, 3], [7, 8]]
+    most = 1e4 if dtype != "float16" else min(1e4, 1e3 * T)
+    for g in (1e-3, 1.0, 5.0, 655.0, 1e4):
+        g = min(g, most)
+        _check_grad(sampler, x, T, tokens, [[0.5 * g, -0.25 * g]] * 6, [g, -g, g, g, g, -g])
+        _check_grad(sampler, x, T, None, None, [g, -g, g, g, g, -g])
