@@ -1196,12 +1196,13 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
   if (live) fetch(v);  // on their way while the row's numbers are read
   const double S = live ? A.row_sum[r] : 0.0;
   double G = 0.0;
-  for (int t = 0; t < A.n_tok; t++) G += (double)s_g[t];
   const double gH = A.g_ent ? (double)A.g_ent[r] : 0.0;
-  const bool zero = S == 0.0 || (G == 0.0 && gH == 0.0);  // padded, all -Inf, or nothing to pass on
-  bool tokens_too = !zero;
-  if (zero && S != 0.0)
-    for (int t = 0; t < A.n_tok; t++) tokens_too |= s_g[t] != 0.f;  // gradients that cancel in G
+  bool some = gH != 0.0;  // not G: gradients that cancel in it are the tokens' own, and NaN in a NaN row
+  for (int t = 0; t < A.n_tok; t++) {
+    G += (double)s_g[t];
+    some |= s_g[t] != 0.f;
+  }
+  const bool zero = S == 0.0 || !some;  // padded, all -Inf, or nothing to pass on
   const float m = (float)(A.row_max[r] * A.T);  // the row's largest logit, exact
   const double log_s = log(S), H = gH != 0.0 ? (double)A.entropy[r] : 0.0;
   const double k = -A.rT / S;
@@ -1236,7 +1237,7 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
     v += kGradThreads * kGradVecs;
     fetch(v);
   }
-  if (!tokens_too) return;
+  if (zero) return;
   __syncthreads();
   for (int t = threadIdx.x; t < A.n_tok; t += kGradThreads) {
     const int y = s_y[t];

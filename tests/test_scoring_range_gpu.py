@@ -110,3 +110,28 @@ def test_score_gradient_of_masked_rows_at_any_temperature(sampler, dtype, T):
         g = min(g, most)
         _check_grad(sampler, x, T, tokens, [[0.5 * g, -0.25 * g]] * 6, [g, -g, g, g, g, -g])
         _check_grad(sampler, x, T, None, None, [g, -g, g, g, g, -g])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_score_gradients_that_cancel_in_rows_without_a_distribution(sampler, dtype):
+    """Token gradients that add up to 0: NaN for a NaN or +Inf logit (0 times a NaN probability), 0 for padding and
+    for -Inf alone; all gradients 0: 0."""
+    import torch
+
+    V = 1501
+    x = _block(np.random.default_rng(4), 6, V, dtype, 1, 1)
+    x[0, 17] = float("nan")
+    x[1, 9] = float("inf")
+    x[2] = -float("inf")
+    x[3, 3] = float("nan")
+    x[5, 17] = float("nan")
+    tok = torch.tensor([[3, 4]] * 3 + [[-1, V]] + [[3, 4]] * 2, dtype=torch.int32, device="cuda")
+    g = torch.tensor([[0.5, -0.5]] * 5 + [[0.0, 0.0]], device="cuda")
+    o = sampler.logprobs(x, tok, entropy=True, stats=True)
+    for g_ent in (None, torch.zeros(6, device="cuda")):
+        dx = sampler.logprobs_backward(x, tok, o.row_max, o.row_sum, g, g_ent, o.entropy if g_ent is not None else None)
+        assert bool(dx[:2].isnan().all())
+        assert bool((dx[[2, 3, 5]] == 0).all())
+        want = torch.zeros(V, dtype=x.dtype, device="cuda")
+        want[3], want[4] = 0.5, -0.5
+        assert torch.equal(dx[4], want)
