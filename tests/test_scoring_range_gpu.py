@@ -1,9 +1,10 @@
 """Scoring operators over the whole range of finite logits and of temperatures, against the 64-bit oracle within
-the bounds that it derives."""
+the bounds that it derives, and over offsets beyond 32 bits."""
 import numpy as np
 import pytest
 
-from test_scoring_gpu import _block, _check_distill, _check_grad, _check_score, _np, _torch
+import scoring_oracle as O
+from test_scoring_gpu import _block, _check_distill, _check_grad, _check_score, _near, _np, _torch
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +136,61 @@ def test_score_gradients_that_cancel_in_rows_without_a_distribution(sampler, dty
         want = torch.zeros(V, dtype=x.dtype, device="cuda")
         want[3], want[4] = 0.5, -0.5
         assert torch.equal(dx[4], want)
+
+
+@pytest.mark.parametrize("kind", ["logits", "logprobs"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [0.00011, 0.01, 0.3, 30.0, 10000.0])
+def test_distill_of_masked_rows_at_any_temperature(sampler, kind, dtype, T):
+    import torch
+
+    V, K = 2051, 6
+    low = torch.finfo(_torch(dtype)).min
+    x = _block(np.random.default_rng(8), 5, V, dtype, 1, 1)
+    ids = [[1, 3, 501, 77, V - 2, -1]] * 5
+    x[0, ::2] = -float("inf")
+    if dtype == "float16" or T >= 1:  # elsewhere (lowest - largest) / T is no fp32 number
+        x[1, ::2] = low
+        x[2, 600:] = low
+    x[3, 600:V - 3] = -float("inf")
+    v = np.log(np.array([[0.3, 0.25, 0.2, 0.1, 0.05, 0.9]] * 5))
+    _check_distill(sampler, x, T, ids, v.tolist(), kind, [T, 0.5 * T, -T, T, 0.0])
+
+
+def test_gradients_beyond_32_bit_offsets(sampler):
+    """Rows 2^27 elements apart, the last ones beyond 2^31 elements: gradients written over the logits and beside
+    them equal those of the same rows packed."""
+    import torch
+
+    B, V, ld = 20, 1003, (1 << 27) + 1
+    packed = torch.randn(B, V, device="cuda").bfloat16()
+    buf = torch.empty((B - 1) * ld + V, dtype=torch.bfloat16, device="cuda")
+    x = buf.as_strided((B, V), (ld, 1))
+    tok = torch.randint(0, V, (B,), dtype=torch.int32, device="cuda")
+    g, ge = torch.randn(B, device="cuda"), torch.randn(B, device="cuda")
+    o = sampler.logprobs(packed, tok, entropy=True, stats=True, top_n=9)
+    want = sampler.logprobs_backward(packed, tok, o.row_max, o.row_sum, g, ge, o.entropy)
+    x.copy_(packed)
+    over = sampler.logprobs_backward(x, tok, o.row_max, o.row_sum, g, ge, o.entropy, out=x)
+    assert over.data_ptr() == x.data_ptr() and torch.equal(over, want)
+    beside = sampler.logprobs_backward(packed, tok, o.row_max, o.row_sum, g, ge, o.entropy, out=x.zero_())
+    assert torch.equal(beside, want)
+    x.copy_(torch.randn(B, V, device="cuda"))
+    ids, v = o.top_ids, o.top_logprobs
+    X, loss = _np(x), sampler.distill_loss(x, ids, v)
+    l1, d1 = sampler.distill_grad(x, ids, v, g)
+    l2, d2 = sampler.distill_grad(x, ids, v, g, out=x)
+    assert d2.data_ptr() == x.data_ptr() and torch.equal(d2, d1)
+    assert torch.equal(l1, loss) and torch.equal(l2, loss)
+    for r in range(B):
+        wl, bl, wd, bd = O.distill(X[r], 1.0, ids[r].tolist(), _np(v[r]), "logprobs", float(g[r]), "bfloat16")
+        _near([_np(loss)[r]], [wl], bl, ("loss", r))
+        _near(_np(d1[r]), wd, bd, ("dlogits", r))
+    # the scores' gradient against the definition
+    lp = torch.log_softmax(packed.double(), 1)
+    h = -(lp.exp() * lp).sum(1, keepdim=True)
+    d = -lp.exp() * (g[:, None].double() + ge[:, None].double() * (lp + h))
+    d.scatter_add_(1, tok[:, None].long(), g[:, None].double())
+    # one rounding to bf16, and some hundred fp32 roundings of terms of at most |g| + |g_H| (|log p| + H)
+    near = 2.0 ** -8 * d.abs() + 2.0 ** -16 * (g.abs() + 20 * ge.abs())[:, None]
+    assert bool(((want.double() - d).abs() <= near).all())
