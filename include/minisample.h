@@ -375,7 +375,7 @@ int ms_logprobs_backward(ms_ctx* ctx, const void* logits, int dtype, int64_t B, 
 
 /*
  * Distillation: the divergence of the student's softmax(z) from a teacher known
- * by its top ids, and its gradient, from one read of the logits.
+ * by its top ids, and its gradient, in one launch.
  *   ids, values  [B, K] int32 / float, 1 <= K <= 256; an id outside [0, V) is
  *            absent, and a row without a present id is padding (loss 0,
  *            gradient 0, logits not read)
@@ -391,8 +391,10 @@ int ms_logprobs_backward(ms_ctx* ctx, const void* logits, int dtype, int64_t B, 
  *   weight   [B] or NULL (1): dlogits is weight times the gradient of loss; a
  *            row of weight 0 gets gradient 0.  loss is not weighted.
  *   dlogits  [B, dld] of `dtype` or NULL; as for ms_logprobs_backward
- * An id that is listed twice has the sum of both masses; the student's
- * probability of it counts once.
+ * Every entry is a term of the loss, an id that is listed twice two terms, each
+ * with its own mass: sum_j q_j log(q_id / q_j) less than for one entry of both
+ * masses q_id (a constant, so the gradient, where q_id stands, is the same; the
+ * loss can be negative).  The student's probability of it counts once.
  */
 #define MS_TEACHER_LOGITS   0
 #define MS_TEACHER_LOGPROBS 1

@@ -194,3 +194,35 @@ def test_gradients_beyond_32_bit_offsets(sampler):
     # one rounding to bf16, and some hundred fp32 roundings of terms of at most |g| + |g_H| (|log p| + H)
     near = 2.0 ** -8 * d.abs() + 2.0 ** -16 * (g.abs() + 20 * ge.abs())[:, None]
     assert bool(((want.double() - d).abs() <= near).all())
+
+
+@pytest.mark.parametrize("kind", ["logits", "logprobs"])
+def test_distill_of_an_id_listed_twice(sampler, kind):
+    """Against the same teacher with the id listed once with both masses: the gradient is the same, the loss less by
+    sum_j q_j log(q_id / q_j)."""
+    import torch
+
+    V, T = 1203, 1.5
+    x = _block(np.random.default_rng(3), 2, V, "float32")
+    q = np.array([0.3, 0.2, 0.15, 0.1])                         # 7 twice, in one row next to one another
+    ids = torch.tensor([[7, 40, 7, 1200], [40, 7, 7, 3]], dtype=torch.int32, device="cuda")
+    both = [0.45, 0.35]
+    less = [0.3 * np.log(0.45 / 0.3) + 0.15 * np.log(0.45 / 0.15), 0.2 * np.log(0.35 / 0.2) + 0.15 * np.log(0.35 / 0.15)]
+    if kind == "logits":
+        less = [v / q.sum() for v in less]
+    scale = T if kind == "logits" else 1.0                      # the logits' softmax is taken at T
+    v = torch.tensor(np.log(np.array([q, q])) * scale, dtype=torch.float32, device="cuda")
+    one, w = ids.clone(), v.clone()
+    one[0, 2] = one[1, 2] = -1
+    w[0, 0], w[1, 1] = np.log(both[0]) * scale, np.log(both[1]) * scale
+    loss, dx = sampler.distill_grad(x, ids, v, temperature=T, kind=kind)
+    l1, d1 = sampler.distill_grad(x, one, w, temperature=T, kind=kind)
+    # the masses differ by the rounding of their logarithms (of at most 3, half a step 2^-24 of it), the loss by that
+    # of its terms (of at most 16 here), the gradient by a mass's
+    np.testing.assert_allclose(_np(l1) - _np(loss), less, atol=2.0 ** -24 * 3 * 2 * 16)
+    np.testing.assert_allclose(_np(dx), _np(d1), atol=2.0 ** -24 * 3 * 2)
+    # a row's own distribution with an id's mass in two halves: no divergence but that of the halves
+    z = torch.log(torch.tensor([[0.5, 0.25, 0.25]], device="cuda"))
+    halves = torch.log(torch.tensor([[0.25, 0.25, 0.25, 0.25]], device="cuda"))
+    own = sampler.distill_loss(z, torch.tensor([[0, 0, 1, 2]], dtype=torch.int32, device="cuda"), halves, kind=kind)
+    np.testing.assert_allclose(_np(own), [0.5 * np.log(0.5)], atol=2.0 ** -20)
