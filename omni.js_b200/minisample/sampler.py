@@ -41,6 +41,16 @@ def _is_torch(x) -> bool:
     return type(x).__module__.startswith("torch")
 
 
+def _written(t) -> None:
+    """Tells autograd that a caller's tensor was written, which goes by its
+    address: a graph that saved it raises then, as for torch's own operations in
+    place, and does not go on with what is there now."""
+    import torch
+
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 _SCORING = None
 
 
@@ -285,6 +295,8 @@ class Sampler:
             rc = self._L.ms_sample(self._ctx, logits.data_ptr(), B, V, ld, hp, hop, ctypes.byref(p), up,
                                    ids.data_ptr(), ctypes.byref(D) if D is not None else None, flags,
                                    _stream_handle(st))
+        if out is not None:
+            _written(out)
         self._check(rc)
         if diag:
             return ids, keep
@@ -350,6 +362,8 @@ class Sampler:
                                           None if u is None else u.data_ptr(), ids.data_ptr(),
                                           ctypes.byref(D) if D is not None else None, R,
                                           _stream_handle(st))
+        if out is not None:
+            _written(out)
         self._check(rc)
         if diag:
             return ids, keep

@@ -14,6 +14,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
+from .sampler import _written
 
 _DTYPES = {torch.float32: N.MS_F32, torch.bfloat16: N.MS_BF16, torch.float16: N.MS_F16}
 _KINDS = {"logits": N.MS_TEACHER_LOGITS, "logprobs": N.MS_TEACHER_LOGPROBS}
@@ -177,6 +178,8 @@ def logprobs_backward(s, logits, tokens, row_max, row_sum, g_logprobs=None, g_en
     s._check(s._L.ms_logprobs_backward(s._ctx, logits.data_ptr(), dtype, B, V, ld, float(temperature), _p(tok),
                                        n, row_max.data_ptr(), row_sum.data_ptr(), _p(entropy), _p(g_logprobs),
                                        _p(g_entropy), dx.data_ptr(), dx.stride(0), _current(s)))
+    if out is not None:
+        _written(out)
     return dx
 
 
@@ -234,4 +237,7 @@ def distill_grad(s, logits, teacher_ids, teacher_values, weight=None, *, tempera
                                         kind=kind, out=out))
     _block(s, logits)
     dx = _grad_out(s, logits, out)
-    return _distill(s, logits, teacher_ids, teacher_values, weight, temperature, kind, True, dx), dx
+    loss = _distill(s, logits, teacher_ids, teacher_values, weight, temperature, kind, True, dx)
+    if out is not None:
+        _written(out)
+    return loss, dx

@@ -1,0 +1,64 @@
+"""What autograd sees of the scoring calls: blocks written in place, outputs, derivatives that they do not have."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _teacher(s, B, V, n=8):
+    import torch
+
+    o = s.logprobs(torch.randn(B, V, device="cuda"), top_n=n)
+    return o.top_ids, o.top_logprobs
+
+
+@pytest.mark.parametrize("forward", ["logprobs", "distill_loss"])
+@pytest.mark.parametrize("over", ["logprobs_backward", "distill_grad"])
+def test_a_gradient_written_over_saved_logits_is_noticed(sampler, forward, over):
+    """Autograd raises, as for any block that is modified in place, where it would use the overwritten logits."""
+    import torch
+
+    x = torch.randn(5, 301, device="cuda", requires_grad=True)
+    tok = torch.randint(0, 301, (5,), device="cuda", dtype=torch.int32)
+    ids, v = _teacher(sampler, 5, 301)
+    y = (sampler.logprobs(x, tok).logprobs if forward == "logprobs" else sampler.distill_loss(x, ids, v)).sum()
+    before = x._version
+    with torch.no_grad():
+        if over == "logprobs_backward":
+            o = sampler.logprobs(x, tok, stats=True)
+            sampler.logprobs_backward(x, tok, o.row_max, o.row_sum, torch.ones(5, device="cuda"), out=x)
+        else:
+            sampler.distill_grad(x, ids, v, out=x)
+    assert x._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_ids_drawn_over_saved_tokens_are_noticed(sampler):
+    import torch
+
+    from minisample import SampleParams
+
+    x = torch.randn(5, 301, device="cuda", requires_grad=True)
+    u = torch.rand(5, dtype=torch.float64, device="cuda")
+    ids = sampler.sample(x.detach(), SampleParams(), u=u, sync=False)
+    y = sampler.logprobs(x, ids).logprobs.sum()
+    sampler.sample(x.detach(), SampleParams(), u=u, out=ids, sync=False)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_gradients_written_to_a_block_of_inference_mode(sampler):
+    """Blocks without a version counter are taken as they were."""
+    import torch
+
+    from minisample import SampleParams
+
+    with torch.inference_mode():
+        x = torch.randn(5, 301, device="cuda")
+        ids, v = _teacher(sampler, 5, 301)
+        loss, dx = sampler.distill_grad(x, ids, v)
+        l2, d2 = sampler.distill_grad(x.clone(), ids, v, out=torch.empty_like(x))
+        assert torch.equal(loss, l2) and torch.equal(dx, d2)
+        drawn = torch.empty(5, dtype=torch.int32, device="cuda")
+        u = torch.rand(5, dtype=torch.float64, device="cuda")
+        assert torch.equal(sampler.sample(x, SampleParams(), u=u, out=drawn), sampler.sample(x, SampleParams(), u=u))
