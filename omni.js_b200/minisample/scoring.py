@@ -128,11 +128,13 @@ def _logprobs(s, x, tokens, temperature, top_n, entropy, stats):
 
 class _LogProbsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, s, tokens, temperature, top_n, entropy):
+    def forward(ctx, x, s, tokens, temperature, top_n, entropy, stats):
         o = _logprobs(s, x, tokens, temperature, top_n, entropy, True)
         ctx.save_for_backward(x, tokens, o.row_max, o.row_sum, o.entropy)
         ctx.s, ctx.temperature = s, temperature
         ctx.set_materialize_grads(False)
+        if not stats:  # the backward pass's, not the caller's
+            o = o._replace(row_max=None, row_sum=None)
         ctx.mark_non_differentiable(*(t for t in (o.top_ids, o.top_logprobs, o.row_max, o.row_sum) if t is not None))
         return tuple(o)
 
@@ -141,10 +143,10 @@ class _LogProbsFn(torch.autograd.Function):
     def backward(ctx, g_lp, g_ent, *_):
         x, tokens, mx, sm, ent = ctx.saved_tensors
         if g_lp is None and g_ent is None:
-            return (None,) * 6
+            return (None,) * 7
         dx = logprobs_backward(ctx.s, x, tokens, mx, sm, g_lp, g_ent, ent if g_ent is not None else None,
                                temperature=ctx.temperature)
-        return (dx,) + (None,) * 5
+        return (dx,) + (None,) * 6
 
 
 def logprobs(s, logits, tokens=None, *, temperature=1.0, top_n=0, entropy=False, stats=False, stream=None):
@@ -152,8 +154,9 @@ def logprobs(s, logits, tokens=None, *, temperature=1.0, top_n=0, entropy=False,
         return _on(s, stream, (logits, tokens),
                    lambda: logprobs(s, logits, tokens, temperature=temperature, top_n=top_n, entropy=entropy,
                                     stats=stats))
-    if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
-        return LogProbs(*_LogProbsFn.apply(logits, s, tokens, temperature, top_n, entropy))
+    if (isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled()
+            and (tokens is not None or entropy)):  # the outputs that carry gradients
+        return LogProbs(*_LogProbsFn.apply(logits, s, tokens, temperature, top_n, entropy, stats))
     return _logprobs(s, logits, tokens, temperature, top_n, entropy, stats)
 
 

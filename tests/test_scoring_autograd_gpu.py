@@ -62,3 +62,21 @@ def test_gradients_written_to_a_block_of_inference_mode(sampler):
         drawn = torch.empty(5, dtype=torch.int32, device="cuda")
         u = torch.rand(5, dtype=torch.float64, device="cuda")
         assert torch.equal(sampler.sample(x, SampleParams(), u=u, out=drawn), sampler.sample(x, SampleParams(), u=u))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_outputs_that_were_not_asked_for_are_none(sampler, grad):
+    import torch
+
+    x = torch.randn(3, 301, device="cuda", requires_grad=grad)
+    tok = torch.zeros(3, dtype=torch.int32, device="cuda")
+    o = sampler.logprobs(x, tok)
+    assert [v is None for v in o] == [False, True, True, True, True, True]
+    o = sampler.logprobs(x, top_n=2, stats=True)
+    assert [v is None for v in o] == [True, True, False, False, False, False]
+    o = sampler.logprobs(x, entropy=True)
+    assert [v is None for v in o] == [True, False, True, True, True, True]
+    if grad:
+        (g,) = torch.autograd.grad(o.entropy.sum(), x)
+        assert g.shape == x.shape
+    assert all(v is None for v in sampler.logprobs(x))
