@@ -156,7 +156,7 @@ class Sampler:
         An id outside [0, V) is no token (log-probability 0); a row with no
         token at all is padding (outputs 0, ids -1).  Differentiable: with
         logits.requires_grad, logprobs and entropy carry gradients (top_ids and
-        top_logprobs do not).  Asynchronous, on `stream` or the current stream
+        top_logprobs do not), in reverse mode only.  Asynchronous, on `stream` or the current stream
         (ms_logprobs)."""
         return _scoring().logprobs(self, logits, tokens, temperature=temperature, top_n=top_n, entropy=entropy,
                                    stats=stats, stream=stream)

@@ -12,6 +12,7 @@ import ctypes
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from .sampler import _written
@@ -48,6 +49,13 @@ def _block(s, x, what="logits"):
     if x.get_device() != s.device_index:
         raise ValueError(f"{what} is on cuda:{x.get_device()}, the sampler on cuda:{s.device_index}")
     return dtype, B, V, ld
+
+
+def _no_tangent(x):
+    """Refuses a dual tensor: the calls have no forward-mode derivatives, and read
+    the primal by its address."""
+    if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError("logits have a tangent: the scoring calls have no forward-mode derivatives")
 
 
 def _rows(t, name, x, dtype, shape):
@@ -154,6 +162,7 @@ def logprobs(s, logits, tokens=None, *, temperature=1.0, top_n=0, entropy=False,
         return _on(s, stream, (logits, tokens),
                    lambda: logprobs(s, logits, tokens, temperature=temperature, top_n=top_n, entropy=entropy,
                                     stats=stats))
+    _no_tangent(logits)
     if (isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled()
             and (tokens is not None or entropy)):  # the outputs that carry gradients
         return LogProbs(*_LogProbsFn.apply(logits, s, tokens, temperature, top_n, entropy, stats))
@@ -166,6 +175,7 @@ def logprobs_backward(s, logits, tokens, row_max, row_sum, g_logprobs=None, g_en
         return _on(s, stream, (logits, tokens, row_max, row_sum, g_logprobs, g_entropy, entropy, out),
                    lambda: logprobs_backward(s, logits, tokens, row_max, row_sum, g_logprobs, g_entropy, entropy,
                                              temperature=temperature, out=out))
+    _no_tangent(logits)
     dtype, B, V, ld = _block(s, logits)
     tok, n = _tokens(tokens, logits)
     row_max = _rows(row_max, "row_max", logits, torch.float64, (B,))
@@ -227,6 +237,7 @@ def distill_loss(s, logits, teacher_ids, teacher_values, *, temperature=1.0, kin
     if stream is not None:
         return _on(s, stream, (logits, teacher_ids, teacher_values),
                    lambda: distill_loss(s, logits, teacher_ids, teacher_values, temperature=temperature, kind=kind))
+    _no_tangent(logits)
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return _DistillFn.apply(logits, s, teacher_ids, teacher_values, temperature, kind)
     return _distill(s, logits, teacher_ids, teacher_values, None, temperature, kind, True, None)
@@ -238,6 +249,7 @@ def distill_grad(s, logits, teacher_ids, teacher_values, weight=None, *, tempera
         return _on(s, stream, (logits, teacher_ids, teacher_values, weight, out),
                    lambda: distill_grad(s, logits, teacher_ids, teacher_values, weight, temperature=temperature,
                                         kind=kind, out=out))
+    _no_tangent(logits)
     _block(s, logits)
     dx = _grad_out(s, logits, out)
     loss = _distill(s, logits, teacher_ids, teacher_values, weight, temperature, kind, True, dx)

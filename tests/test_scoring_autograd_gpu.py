@@ -80,3 +80,26 @@ def test_outputs_that_were_not_asked_for_are_none(sampler, grad):
         (g,) = torch.autograd.grad(o.entropy.sum(), x)
         assert g.shape == x.shape
     assert all(v is None for v in sampler.logprobs(x))
+
+
+def test_forward_mode_is_refused(sampler):
+    """The calls have no forward derivatives: a tangent is not dropped without a word."""
+    import torch
+    import torch.autograd.forward_ad as fwad
+
+    x, t = torch.randn(3, 301, device="cuda"), torch.randn(3, 301, device="cuda")
+    tok = torch.zeros(3, dtype=torch.int32, device="cuda")
+    ids, v = _teacher(sampler, 3, 301)
+    o = sampler.logprobs(x, tok, stats=True)
+    g = torch.ones(3, device="cuda")
+    with fwad.dual_level():
+        for z in (fwad.make_dual(x, t), fwad.make_dual(x.clone().requires_grad_(), t)):
+            for call in (lambda: sampler.logprobs(z, tok), lambda: sampler.distill_loss(z, ids, v),
+                         lambda: sampler.logprobs_backward(z, tok, o.row_max, o.row_sum, g),
+                         lambda: sampler.distill_grad(z, ids, v)):
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call()
+        assert torch.equal(sampler.logprobs(x, tok).logprobs, o.logprobs)  # no tangent: as ever
+    for call in (lambda z: sampler.logprobs(z, tok).logprobs, lambda z: sampler.distill_loss(z, ids, v)):
+        with pytest.raises((ValueError, RuntimeError)):
+            torch.func.jvp(call, (x,), (t,))
