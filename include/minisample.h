@@ -21,8 +21,9 @@
  *     to a CPU implementation.
  *   - The caller owns every buffer.  The logits are never modified (the
  *     reference copies them first, src/generation.js:72).
- *   - A context is used by one host thread at a time.  Its scratch memory is
- *     shared by every call made on it: two ms_sample calls whose kernels can
+ *   - A context is used by one host thread at a time (the scoring calls may
+ *     come from several).  Its scratch memory is shared by every other call
+ *     made on it: two ms_sample calls whose kernels can
  *     run at the same time (MS_DEVICE_PTRS calls on two streams with nothing
  *     ordering them) race on that scratch.  Order such calls on one stream, or
  *     give each stream its own context.
@@ -315,8 +316,9 @@ int ms_merge_records(ms_ctx* ctx, const void* records, int64_t B, int64_t G, int
  *
  * All three calls take device pointers on the context's first device, run on
  * `stream` (NULL = the ctx stream) asynchronously, keep nothing between calls
- * and use no scratch memory: calls on several streams, and captured and
- * replayed ones, do not disturb one another.
+ * and use no scratch memory: calls on several streams, of several host threads
+ * (ms_last_error is the last failed one's), and captured and replayed ones, do
+ * not disturb one another.
  *
  * Common arguments:
  *   logits   [B, ld] of `dtype` (MS_F32, MS_BF16 or MS_F16), ld >= V (row

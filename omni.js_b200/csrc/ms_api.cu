@@ -6,7 +6,6 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
-#include <string>
 #include <algorithm>
 #include <array>
 #include <vector>
@@ -42,6 +41,7 @@ struct DevState {
   std::vector<std::array<cudaEvent_t, 3>> prof_pending;  // MS_PROFILE calls not yet read
   std::vector<std::array<cudaEvent_t, 3>> prof_free;
   int64_t launches = 0;  // kernels launched on this device
+  int64_t score_launches = 0;  // the scoring calls', which several host threads may make: counted atomically
 };
 
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
@@ -140,18 +140,23 @@ ScratchLayout scratch_layout(int64_t B, int64_t V, const Plan& P) {
 
 struct ms_ctx {
   std::vector<DevState> devs;
-  std::string err = "no error";
+  // the last failed call's message, always terminated; the lock is the writers'
+  char err[512] = "no error";
+  std::mutex err_mu;
   long long inject_wait = 0;   // ms_debug_inject(MS_INJECT_WAIT): cycles, next call only
   bool inject_alloc = false;   // ms_debug_inject(MS_INJECT_ALLOC): fail the next allocation
 };
 
 static int fail(ms_ctx* c, int code, const char* fmt, ...) {
-  char buf[512];
+  char buf[sizeof c->err];
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
-  if (c) c->err = buf;
+  if (c) {
+    std::lock_guard<std::mutex> lock(c->err_mu);
+    strcpy(c->err, buf);
+  }
   return code;
 }
 
@@ -285,7 +290,7 @@ int ms_destroy(ms_ctx* c) {
   return MS_OK;
 }
 
-const char* ms_last_error(ms_ctx* c) { return c ? c->err.c_str() : "null context"; }
+const char* ms_last_error(ms_ctx* c) { return c ? c->err : "null context"; }
 
 int ms_profile_read(ms_ctx* c, double* stream_ms, double* finalize_ms, int64_t* calls) {
   if (!c) return MS_ERR_ARG;
@@ -319,7 +324,7 @@ int ms_profile_read(ms_ctx* c, double* stream_ms, double* finalize_ms, int64_t* 
 int ms_launch_count(ms_ctx* c, int64_t* kernels) {
   if (!c || !kernels) return MS_ERR_ARG;
   int64_t n = 0;
-  for (auto& s : c->devs) n += s.launches;
+  for (auto& s : c->devs) n += s.launches + __atomic_load_n(&s.score_launches, __ATOMIC_RELAXED);
   *kernels = n;
   return MS_OK;
 }
@@ -843,7 +848,7 @@ extern "C" int ms_logprobs(ms_ctx* ctx, const void* logits, int dtype, int64_t B
   OnDevice on(s.device);
   MS_CUDA(ctx, on.err);
   MS_CUDA(ctx, ms::launch_logprobs(A, dtype, stream ? (cudaStream_t)stream : s.stream));
-  s.launches += 1;
+  __atomic_fetch_add(&s.score_launches, 1, __ATOMIC_RELAXED);
   return MS_OK;
 }
 
@@ -881,7 +886,7 @@ extern "C" int ms_logprobs_backward(ms_ctx* ctx, const void* logits, int dtype, 
   OnDevice on(s.device);
   MS_CUDA(ctx, on.err);
   MS_CUDA(ctx, ms::launch_logprobs_backward(A, dtype, stream ? (cudaStream_t)stream : s.stream));
-  s.launches += 1;
+  __atomic_fetch_add(&s.score_launches, 1, __ATOMIC_RELAXED);
   return MS_OK;
 }
 
@@ -913,6 +918,6 @@ extern "C" int ms_distill(ms_ctx* ctx, const void* logits, int dtype, int64_t B,
   OnDevice on(s.device);
   MS_CUDA(ctx, on.err);
   MS_CUDA(ctx, ms::launch_distill(A, dtype, stream ? (cudaStream_t)stream : s.stream));
-  s.launches += 1;
+  __atomic_fetch_add(&s.score_launches, 1, __ATOMIC_RELAXED);
   return MS_OK;
 }
