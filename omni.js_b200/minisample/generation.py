@@ -73,6 +73,12 @@ def normalize_options(options: dict | None) -> dict:
     }
 
 
+def _without_logprobs(opts: dict) -> dict:
+    if opts["logprobs"] is not None:
+        raise ValueError("logprobs are returned by generate_tokens_device only")
+    return opts
+
+
 def params_of(opts: dict) -> SampleParams:
     return SampleParams(bool(opts["do_sample"]), float(opts["temperature"]), int(opts["top_k"]),
                         float(opts["top_p"]), float(opts["repetition_penalty"]))
@@ -106,7 +112,7 @@ def last_token_logits(model, input_ids, cache):
 
 
 def generate_tokens(model, input_ids, options=None, rand=_random.random):
-    opts = normalize_options(options)
+    opts = _without_logprobs(normalize_options(options))
     cache = model.make_cache()
     try:
         generated = []
@@ -125,7 +131,7 @@ def generate_tokens(model, input_ids, options=None, rand=_random.random):
 
 
 async def generate_async(model, input_ids, options=None, rand=_random.random):
-    opts = normalize_options(options)
+    opts = _without_logprobs(normalize_options(options))
     tick = (options or {}).get("tick")
     cache = model.make_cache()
     try:
@@ -157,7 +163,7 @@ def generate_tokens_batch(model, input_ids_batch, options=None, rands=None):
     uniforms (one per sampled step of that row, none when greedy), so row i
     gets the ids generate_tokens would give it with rands[i].  `model` is one
     model for every row, or a list of one per row."""
-    opts = normalize_options(options)
+    opts = _without_logprobs(normalize_options(options))
     B = len(input_ids_batch)
     models = model if isinstance(model, (list, tuple)) else [model] * B
     rands = rands if rands is not None else [_random.random] * B
