@@ -326,6 +326,7 @@ int ms_merge_records(ms_ctx* ctx, const void* records, int64_t B, int64_t G, int
  *            1 <= V <= 65535 * 16384, B <= 2^31 - 1
  *   temperature  z = logits / temperature; 0.0001 < temperature <= 10000
  *   a -Inf logit is an id that cannot be chosen: probability 0
+ * Every other array is aligned to its elements too.
  * Rows without a distribution:
  *   a NaN or +Inf logit: the row's outputs and gradients are NaN, its ids -1
  *   every logit -Inf: log-probabilities -Inf, entropy 0, no alternatives,

@@ -831,6 +831,7 @@ extern "C" int ms_logprobs(ms_ctx* ctx, const void* logits, int dtype, int64_t B
   if (const char* e = ms::bad_logprobs(logits, dtype, B, V, ld, temperature, tokens, n_tokens, top_n, out))
     return fail(ctx, MS_ERR_ARG, "ms_logprobs: %s", e);
   if (B == 0) return MS_OK;
+  if (const char* e = ms::bad_scores(*out)) return fail(ctx, MS_ERR_ARG, "ms_logprobs: %s", e);
   DevState& s = ctx->devs[0];
   ms::ScoreArgs A;
   memset(&A, 0, sizeof A);
@@ -894,7 +895,8 @@ extern "C" int ms_distill(ms_ctx* ctx, const void* logits, int dtype, int64_t B,
                           double temperature, const int32_t* ids, const float* values, int32_t K, int kind,
                           const float* weight, float* loss, void* dlogits, int64_t dld, void* stream) {
   if (!ctx) return MS_ERR_ARG;
-  if (const char* e = ms::bad_distill(logits, dtype, B, V, ld, temperature, ids, values, K, kind, loss, dlogits, dld))
+  if (const char* e = ms::bad_distill(logits, dtype, B, V, ld, temperature, ids, values, K, kind, loss, dlogits, dld,
+                                        weight))
     return fail(ctx, MS_ERR_ARG, "ms_distill: %s", e);
   if (B == 0) return MS_OK;
   DevState& s = ctx->devs[0];

@@ -1,6 +1,7 @@
 // Argument checks of the scoring calls, without CUDA: each returns NULL or what
 // is wrong with the call.
 #pragma once
+#include <cstddef>
 #include <cstdint>
 
 #include "../../include/minisample.h"
@@ -11,6 +12,8 @@ constexpr int kScoreMax = 256;                      // largest n_tokens, top_n a
 constexpr int64_t kScoreVMax = (int64_t)65535 * 16384;  // ms_sample's limit
 
 inline int64_t elem_bytes(int dtype) { return dtype == MS_F32 ? 4 : 2; }
+
+inline bool misaligned(const void* p, size_t bytes) { return (uintptr_t)p % bytes != 0; }
 
 inline const char* bad_block(const void* logits, int dtype, int64_t B, int64_t V, int64_t ld, double temperature) {
   if (dtype != MS_F32 && dtype != MS_BF16 && dtype != MS_F16) return "dtype is not MS_F32, MS_BF16 or MS_F16";
@@ -46,6 +49,14 @@ inline const char* bad_logprobs(const void* logits, int dtype, int64_t B, int64_
   if (top_n < 0 || top_n > kScoreMax) return "top_n must be in [0, 256]";
   if (!out) return "out is NULL";
   if (B > 0 && n_tokens > 0 && !tokens) return "tokens is NULL";
+  if (misaligned(tokens, 4)) return "tokens is not aligned to an element";
+  return nullptr;
+}
+
+inline const char* bad_scores(const ms_scores& o) {
+  if (misaligned(o.logprobs, 4) || misaligned(o.entropy, 4) || misaligned(o.top_ids, 4) ||
+      misaligned(o.top_logprobs, 4) || misaligned(o.row_max, 8) || misaligned(o.row_sum, 8))
+    return "an output is not aligned to an element";
   return nullptr;
 }
 
@@ -61,12 +72,15 @@ inline const char* bad_logprobs_backward(const void* logits, int dtype, int64_t 
   if (n_tokens == 0 && g_logprobs) return "g_logprobs without tokens";
   if (!row_max || !row_sum) return "row_max/row_sum is NULL";
   if (g_entropy && !entropy) return "g_entropy without entropy";
+  if (misaligned(tokens, 4) || misaligned(row_max, 8) || misaligned(row_sum, 8) || misaligned(entropy, 4) ||
+      misaligned(g_logprobs, 4) || misaligned(g_entropy, 4))
+    return "an input is not aligned to an element";
   return bad_grad(logits, dtype, B, V, ld, dlogits, dld);
 }
 
 inline const char* bad_distill(const void* logits, int dtype, int64_t B, int64_t V, int64_t ld, double temperature,
                                const int32_t* ids, const float* values, int32_t K, int kind, const float* loss,
-                               const void* dlogits, int64_t dld) {
+                               const void* dlogits, int64_t dld, const float* weight = nullptr) {
   if (const char* e = bad_block(logits, dtype, B, V, ld, temperature)) return e;
   if (K < 1 || K > kScoreMax) return "K must be in [1, 256]";
   if (kind != MS_TEACHER_LOGITS && kind != MS_TEACHER_LOGPROBS)
@@ -74,6 +88,8 @@ inline const char* bad_distill(const void* logits, int dtype, int64_t B, int64_t
   if (B == 0) return nullptr;
   if (!ids || !values) return "ids/values is NULL";
   if (!loss && !dlogits) return "loss and dlogits are both NULL";
+  if (misaligned(ids, 4) || misaligned(values, 4) || misaligned(loss, 4) || misaligned(weight, 4))
+    return "ids, values, weight or loss is not aligned to an element";
   return dlogits ? bad_grad(logits, dtype, B, V, ld, dlogits, dld) : nullptr;
 }
 
