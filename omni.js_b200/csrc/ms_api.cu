@@ -906,7 +906,6 @@ extern "C" int ms_distill(ms_ctx* ctx, const void* logits, int dtype, int64_t B,
   A.B = B;
   A.V = (int32_t)V;
   A.ld = B > 1 ? ld : V;
-  A.T = temperature;
   A.rT = 1.0 / temperature;
   A.a = (float)(1.4426950408889634 / temperature);
   A.ids = ids;

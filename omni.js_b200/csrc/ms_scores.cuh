@@ -33,8 +33,8 @@ struct DistillArgs {
   const void* x;          // [B, ld] logits
   int64_t B, ld;
   int32_t V;
-  double T, rT;
-  float a;
+  double rT;              // fp64(1 / T)
+  float a;                // fp32(log2(e) / T)
   const int32_t* ids;     // [B, K]
   const float* values;    // [B, K]
   int32_t K, kind;

@@ -178,7 +178,7 @@ class Sampler:
         missing mass is held against the ids not listed; or "logits", softmaxed
         over the list at this temperature.  Differentiable in the logits; a
         training step that knows its row weights beforehand gets loss and
-        gradient from one pass with distill_grad (ms_distill)."""
+        gradient from one call of distill_grad (ms_distill)."""
         return _scoring().distill_loss(self, logits, teacher_ids, teacher_values, temperature=temperature, kind=kind,
                                        stream=stream)
 
