@@ -1562,7 +1562,8 @@ __global__ void __launch_bounds__(kRowThreads, DistillShape<GRAD>::kCtas) distil
     // finite however little the student gives them.  What this writes for the
     // listed ids is overwritten below.
     const float mo = O.m == -INFINITY ? 0.f : O.m, zo = mo * A.a;
-    double cd = O.s == 0.0 ? 0.0 : wt * (all * (scale / s) - rest / O.s);
+    // Nothing but -Inf outside the list: 0, or NaN in a row whose listed ids make it so.
+    double cd = O.s == 0.0 ? 0.0 * s : wt * (all * (scale / s) - rest / O.s);
     if (!far(zo)) cd *= exp_small(((double)zo - (double)mo * (double)A.a) * 0.693147180559945309417);
     const float c = (float)cd;
     auto term = [&](float x) { return c * ex2_approx(far(zo) ? __fsub_rn(x, mo) * A.a : fmaf(x, A.a, -zo)); };

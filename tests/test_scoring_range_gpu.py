@@ -226,3 +226,18 @@ def test_distill_of_an_id_listed_twice(sampler, kind):
     halves = torch.log(torch.tensor([[0.25, 0.25, 0.25, 0.25]], device="cuda"))
     own = sampler.distill_loss(z, torch.tensor([[0, 0, 1, 2]], dtype=torch.int32, device="cuda"), halves, kind=kind)
     np.testing.assert_allclose(_np(own), [0.5 * np.log(0.5)], atol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["logits", "logprobs"])
+def test_distill_of_a_bad_logit_in_the_list_and_masks_outside(sampler, dtype, kind):
+    """A NaN or +Inf logit at a listed id makes the whole row NaN where every other id is masked, too."""
+    V = 1201
+    x = _block(np.random.default_rng(2), 4, V, dtype, 1, 1)
+    x[:] = -float("inf")
+    x[0, 40] = float("nan")
+    x[1, 40] = float("inf")
+    x[2, [40, 41]] = 1.0
+    x[3, 700] = float("nan")
+    ids, v = [[40, 41, V - 1]] * 3 + [[700, -1, -1]], np.log([[0.5, 0.25, 0.2]] * 4)
+    _check_distill(sampler, x, 1.0, ids, v.tolist(), kind, [1.0, -2.0, 0.5, 1.0])
