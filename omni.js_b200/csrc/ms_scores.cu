@@ -793,7 +793,7 @@ __device__ __forceinline__ void top_gather(const Row<T>& R, const Slice<T>& S, c
 // Tiles come in order of their ids, so an element that only equals the n-th
 // best of earlier tiles loses to it: tiles without a larger one are passed
 // over, which is most of a row that ties by the thousand (10 finite logits
-// among the type's lowest value, top 20, 64 x 128256 fp32: 74 us; each
+// among the type's lowest value, top 20, 64 x 128256 fp32: 73 us; each
 // tile element by element 156).
 template <typename T>
 __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
@@ -859,7 +859,7 @@ __device__ void top_scan(const Row<T>& R, int top_n, TopSmem& sh) {
 // CTAs an SM and steps of their rings: 96 KiB in flight an SM.  Every other load
 // (tokens, the alternatives' second read) waits behind what the rings have asked
 // for.  us of 2048 x 151936 bf16, 512 x 262144 top 64, 333 x 50257 top 3:
-// 102, 130, 16; with 3 steps 102, 128, 17; with 4 (and so 2 CTAs where there are
+// 102, 130, 16 (now 103, 123, 16); with 3 steps 102, 128, 17; with 4 (and so 2 CTAs where there are
 // alternatives) 102, 120, 23; 4 CTAs, at 64 registers, 121, 130, 17; 2 CTAs with
 // 6 steps 112, 125, 21.
 constexpr int kScoreCtas = 3, kScoreDepth = 2;
@@ -1210,7 +1210,7 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(ScoreAr
   const float c1 = (float)(k * gH * A.rT);
   // e (c0 + c1 (x - m)), x - m bounded below where e is 0 already (-256 ln 2 T): masks lie so far
   // off that c1 times their distance is beyond fp32 (T 0.001, g_H 655), and 0 times that NaN.
-  // As -256 / a, a division in every thread, 2048 x 151936 bf16 takes 189 us for 183.
+  // As -256 / a, a division in every thread, a call of 2048 x 151936 bf16 takes 189 us for 183.
   const float lowest = (float)(-177.4 * A.T);
   auto term = [&](float x) {
     const float dd = max_or_nan(__fsub_rn(x, m), lowest);
