@@ -241,3 +241,86 @@ def test_distill_of_a_bad_logit_in_the_list_and_masks_outside(sampler, dtype, ki
     x[3, 700] = float("nan")
     ids, v = [[40, 41, V - 1]] * 3 + [[700, -1, -1]], np.log([[0.5, 0.25, 0.2]] * 4)
     _check_distill(sampler, x, 1.0, ids, v.tolist(), kind, [1.0, -2.0, 0.5, 1.0])
+
+
+def test_largest_vocabulary(sampler):
+    """One row of the largest accepted V: the last id drawn, listed and at the end of the gradient."""
+    import torch
+
+    V = 65535 * 16384
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(1, V, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    best = [V - 1, 7, V // 2 + 3, V - 12345, 1 << 29]
+    x[0, best] = torch.tensor([16.0, 15.5, 15.0, 14.5, 14.0], dtype=x.dtype, device="cuda")
+    s = q = 0.0
+    for part in x[0].split(1 << 26):
+        z = part.double() - 16.0
+        e = z.exp()
+        s, q = s + float(e.sum()), q + float((e * z).sum())
+    log_s, h = np.log(s), np.log(s) - q / s
+    # roundings of the sums if one CTA took the row: 32 terms a step, V / (256 * 32) steps, and those of RowDist
+    eps = (32 + V / (256 * 32) + 117 + 3 * h) * 2.0 ** -24
+    tok = torch.tensor([V - 1], dtype=torch.int32, device="cuda")
+    o = sampler.logprobs(x, tok, top_n=5, entropy=True, stats=True)
+    assert o.top_ids.tolist() == [best]
+    np.testing.assert_allclose(_np(o.top_logprobs)[0], np.array([16.0, 15.5, 15.0, 14.5, 14.0]) - 16.0 - log_s,
+                               rtol=2.0 ** -24, atol=eps)
+    assert float(o.logprobs) == float(o.top_logprobs[0, 0])
+    # an entropy's terms are weighed by their distance from the maximum, of about 16 here
+    np.testing.assert_allclose(float(o.entropy), h, atol=eps * (1 + 20 + h))
+    p = np.exp(_np(x[0, best]) - 16.0 - log_s)
+    one = torch.ones(1, device="cuda")
+    dx = sampler.logprobs_backward(x, tok, o.row_max, o.row_sum, one)
+    want = np.array([1.0, 0, 0, 0, 0]) - p
+    np.testing.assert_allclose(_np(dx[0, best]), want, rtol=2.0 ** -8, atol=eps)
+    del dx
+    ids = torch.tensor([best], dtype=torch.int32, device="cuda")
+    t = np.array([0.5, 0.2, 0.1, 0.1, 0.05])
+    v = torch.tensor(np.log(t)[None], dtype=torch.float32, device="cuda")
+    loss, dd = sampler.distill_grad(x, ids, v, out=x)
+    rest = 1.0 - np.exp(_np(v)).sum()
+    want = (t * (np.log(t) - np.log(p))).sum() + rest * (np.log(rest) - np.log1p(-p.sum()))
+    np.testing.assert_allclose(float(loss), want, rtol=2.0 ** -23, atol=3 * eps)
+    np.testing.assert_allclose(_np(dd[0, best]), p - t, rtol=2.0 ** -8, atol=2 * eps)
+    assert all(bool(part.isfinite().all()) for part in dd[0].split(1 << 26))
+
+
+def test_hundreds_of_thousands_of_short_rows(sampler):
+    """All rows of a batch that every cluster goes through hundreds of times, against torch in 64 bits."""
+    import torch
+
+    B, V, K = 300_007, 5, 2
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(B, V, device="cuda", generator=g)
+    tok = torch.randint(-1, V, (B,), device="cuda", generator=g, dtype=torch.int32)
+    ids = torch.rand(B, V, device="cuda", generator=g).argsort(1)[:, :K].to(torch.int32)
+    ids[::3, 0] = -1
+    ids[::9] = -1
+    v = torch.log_softmax(torch.randn(B, V, device="cuda", generator=g), 1)[:, :K].contiguous()
+    o = sampler.logprobs(x, tok, top_n=3, entropy=True, stats=True)
+    dx = sampler.logprobs_backward(x, tok, o.row_max, o.row_sum, torch.ones(B, device="cuda"))
+    loss, dd = sampler.distill_grad(x, ids, v)
+    lp = torch.log_softmax(x.double(), 1)
+    p, live, at = lp.exp(), tok >= 0, tok.clamp(min=0).long()[:, None]
+    near = 2.0 ** -24 * 140  # the roundings of a row of few ids, over values of order 1 to 10
+    zero = torch.zeros((), dtype=torch.float64, device="cuda")
+    got = [(o.logprobs, torch.where(live, lp.gather(1, at)[:, 0], zero)),
+           (o.entropy, torch.where(live, -(p * lp).sum(1), zero)),
+           (dx, torch.where(live[:, None], torch.zeros_like(p).scatter_(1, at, 1.0) - p, zero))]
+    top = torch.sort(x, dim=1, descending=True, stable=True)
+    assert torch.equal(o.top_ids[live], top.indices[live, :3].int()) and bool((o.top_ids[~live] == -1).all())
+    got.append((o.top_logprobs[live], lp.gather(1, top.indices)[live, :3]))
+    there = ids >= 0
+    q = torch.where(there, v.double().exp(), zero)
+    mass = torch.zeros(B, V + 1, dtype=torch.float64, device="cuda").scatter_(1, torch.where(there, ids, V).long(), q)
+    on = torch.zeros(B, V + 1, dtype=torch.bool, device="cuda").scatter_(1, torch.where(there, ids, V).long(), True)
+    mass, on, rest = mass[:, :V], on[:, :V], 1.0 - q.sum(1)
+    left = torch.where(on, zero, p).sum(1)
+    want = torch.where(there, q * (v.double() - lp.gather(1, ids.clamp(min=0).long())), zero).sum(1)
+    want = want + rest * (rest.log() - left.log())
+    some = there.any(1)
+    got.append((loss, torch.where(some, want, zero)))
+    got.append((dd, torch.where(some[:, None], p - torch.where(on, mass, p * (rest / left)[:, None]), zero)))
+    for i, (a, b) in enumerate(got):
+        off = (a.double() - b).abs()
+        assert bool((off <= near * (1 + b.abs()) + 3 * near).all()), (i, float(off.max()))
